@@ -407,6 +407,130 @@ int mkv_swap_blocks_device_ids(const int64_t* src_ids, const int64_t* dst_ids, i
                                int32_t is_swap_in, const mkv_pool* pool, void* k_swap,
                                void* v_swap, int64_t num_host_blocks, void* stream);
 
+/* ---- 8-bit paged cache ----------------------------------------------------- */
+/* No counterpart in the reference, whose cache is fp16 (MS/worker/model.py:180-190).
+ * The same path -- append, paged decode attention, chunked prefill over the cache --
+ * with K and V held in 8 bits and one power-of-two scale for each (block, layer,
+ * kv head), K and V apart:
+ *
+ *   k       [num_blocks, L, Hkv, 16, D] codes       a token's head dims contiguous
+ *   v       [num_blocks, L, Hkv, D, 16] codes       a head dim's tokens contiguous
+ *   scales  [L, Hkv, num_blocks, 2]     uint8       biased exponents of (K, V)
+ *
+ * A code c stands for c * 2^(scale - 127).  A cache is read with the element type
+ * (dtype) it was written with.  Limits (MKV_EINVAL otherwise): block_size 16,
+ * head_dim 64 or 128, num_q_heads / num_kv_heads from 1 to 16, k, v 16-byte and
+ * scales 2-byte aligned, 1 to 2^31 - 1 blocks. */
+#define MKV_F16       0   /* dtype of q, k, v, o                                  */
+#define MKV_BF16      1
+#define MKV_KV8_E4M3  0   /* kind of the codes: OCP e4m3 (largest 448)            */
+#define MKV_KV8_INT8  1   /* two's complement, -127 .. 127                        */
+#define MKV_ROPE_NONE        0
+#define MKV_ROPE_HALF        1   /* pairs (d, d + R/2), d < R/2                   */
+#define MKV_ROPE_INTERLEAVED 2   /* pairs (2d, 2d + 1), d < R/2                   */
+
+typedef struct mkv_pool8 {
+    void*    k;
+    void*    v;
+    uint8_t* scales;
+    int64_t  num_blocks;
+    int32_t  num_layers;
+    int32_t  num_kv_heads;
+    int32_t  block_size;
+    int32_t  head_dim;
+    int32_t  kind;
+    int32_t  _pad;
+} mkv_pool8;
+
+/* The rows of one step, prefill sequences first: rows prefill_start_locs[b] + t,
+ * t < prefill_lens[b], hold positions prefix_lens[b] + t of sequence seq_ids[b]; row
+ * num_prefill_tokens + i holds position decoding_lens[i] - 1 of sequence
+ * seq_ids[num_prefill_seqs + i].  prefix_lens NULL = 0.  max_prefill_len bounds
+ * prefill_lens on the host.  A sequence appears once in a batch.  A sequence id
+ * outside the table, a table entry that names no block of the pool and positions
+ * beyond the table row hold nothing: they are neither read nor written. */
+typedef struct mkv_batch {
+    const int32_t* block_table;      /* [table_rows, max_blocks_per_seq] */
+    int64_t        max_blocks_per_seq;
+    int64_t        table_rows;
+    const int32_t* seq_ids;
+    const int32_t* prefill_start_locs;
+    const int32_t* prefill_lens;
+    const int32_t* prefix_lens;
+    const int32_t* decoding_lens;
+    int32_t        num_prefill_seqs;
+    int32_t        num_prefill_tokens;
+    int32_t        max_prefill_len;
+    int32_t        num_decoding_seqs;
+} mkv_batch;
+
+int mkv_sizeof_pool8(void);                  /* for binding checks */
+int mkv_sizeof_batch(void);
+
+/* Appends the rows of the batch to the cache, like store_kvcache
+ * (MS/worker/kernels/kvcache_mgmt.py:298-414) does to an fp16 one; k, v :
+ * [rows, Hkv, D], a row k_stride / v_stride elements after the one before.  For the
+ * rows [a, b) a block receives (per head, K and V apart), with M = 448 or 127:
+ *   e = the least exponent >= -126 with max |x| <= M * 2^e; where a > 0, at least
+ *       the exponent the block has, and if that makes it larger the codes of rows
+ *       < a are rounded to the new scale;
+ *   codes = x * 2^-e, rounded to nearest, ties to even.
+ * Rows at or behind b keep their codes.  |x| is clamped to 1.875 * 2^15 (fp16) or
+ * 1.875 * 2^127 (bf16) first; a NaN takes no part in the maximum and is stored as a
+ * NaN (e4m3) or as 0 (int8).
+ * rope != MKV_ROPE_NONE: k is rotated first, in 32 bits and with no rounding before
+ * the codes', and q : [rows, Hq, D] is rotated into q_out (which may be q), by row
+ * `position` of cos_table / sin_table ([num_positions, rotary_dim / 2] fp32); head
+ * dims >= rotary_dim stay as they are.  k itself is not written.  A row whose
+ * position lies outside the tables is not appended and its rotated q is NaN.
+ * rotary_dim: a multiple of 16 up to D.  Pointers and strides in multiples of 16
+ * bytes.  With MKV_ROPE_NONE q, q_out and the tables are ignored. */
+int mkv_store8(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* k,
+               const void* v, int64_t k_stride, int64_t v_stride, int32_t layer, int32_t rope,
+               const void* q, void* q_out, int64_t q_stride, int64_t q_out_stride,
+               int32_t num_q_heads, const float* cos_table, const float* sin_table,
+               int64_t num_positions, int32_t rotary_dim, void* stream);
+
+/* Decode attention over the 8-bit cache: mkv_paged_attn_decode's contract over the
+ * decode rows of the batch.  q, o : [n, Hq, D], rows q_stride / o_stride elements
+ * apart; sequence i attends to its first decoding_lens[i] positions.  A sequence with
+ * nothing to attend to (length 0, or none of its blocks in the pool) gets zeros.
+ * tokens_per_split (a multiple of 64) and max_splits as there; mid_o (fp32
+ * [n, Hq, max_splits, D], 16-byte aligned) and mid_lse (fp32 [n, Hq, max_splits])
+ * may be NULL when max_splits is 1. */
+int mkv_attn8_decode(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* q,
+                     void* o, int64_t q_stride, int64_t o_stride, int32_t num_q_heads,
+                     float softmax_scale, int32_t layer, int32_t tokens_per_split,
+                     int32_t max_splits, void* mid_o, void* mid_lse, void* stream);
+
+/* Chunked prefill over the 8-bit cache: mkv_prefill_attn_paged's contract over the
+ * prefill rows of the batch.  q, o : [num_prefill_tokens, Hq, D]; the row at position
+ * p attends to cached positions <= p of its sequence (append first).  The keys of a
+ * sequence are cut into max_splits ranges of tokens_per_split (a multiple of 64; the
+ * last range takes whatever lies behind it); with max_splits > 1 the partials go
+ * through mid_o (fp32 [num_prefill_tokens, Hq, max_splits, D]) and mid_lse (fp32
+ * [num_prefill_tokens, Hq, max_splits]). */
+int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* q,
+                      void* o, int64_t q_stride, int64_t o_stride, int32_t num_q_heads,
+                      float softmax_scale, int32_t layer, int32_t tokens_per_split,
+                      int32_t max_splits, void* mid_o, void* mid_lse, void* stream);
+
+/* ---- rotary embedding from positions ----------------------------------------- */
+/* rotary_embedding_inplace (MS/worker/kernels/rotary_emb.py:7-58) in the forms it
+ * lacks: half or interleaved pairs, part of the head (rotary_dim <= head_dim, any even
+ * number), rows picked by position out of fp32 tables [num_positions, rotary_dim / 2]
+ * (which may be scaled for long contexts), fp16 or bf16, rows of any stride.
+ *   (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos), in 32 bits, rounded once.
+ * q, k : [num_tokens, H, D]; q_out / k_out may be q / k or must not overlap them; k
+ * may be NULL (num_kv_heads 0).  A row whose position lies outside the tables gets
+ * NaN in its rotated dims. */
+int mkv_rope_positions(int32_t dtype, int32_t layout, const void* q, const void* k, void* q_out,
+                       void* k_out, int64_t q_stride, int64_t k_stride, int64_t q_out_stride,
+                       int64_t k_out_stride, const int32_t* positions, const float* cos_table,
+                       const float* sin_table, int64_t num_positions, int64_t num_tokens,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t rotary_dim, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

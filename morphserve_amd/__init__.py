@@ -6,6 +6,8 @@ Drop-in names (reference file each mirrors):
 * ``worker.kernels.paged_attn.paged_attention``      MorphServe/worker/kernels/paged_attn.py
 * ``worker.kernels.prefill_attn.prefill_attention``  MorphServe/worker/kernels/prefill_attn.py
 * ``worker.kernels.rotary_emb.*``                    MorphServe/worker/kernels/rotary_emb.py (+ fused append)
+* ``kv8_cache.KV8Cache``, ``worker.kernels.kv8.*``   the paged path over a cache in 8 bits: append (+ rotary), decode and
+                                                     chunked prefill attention (no counterpart in the reference)
 * ``worker.kernels.block_mgmt.*``                    MorphServe/worker/kernels/block_mgmt.py
 * ``worker.block_manager.BlockManager``              MorphServe/worker/block_manager.py
 * ``worker.infer_state.LlamaInferState``             MorphServe/worker/infer_state.py
@@ -32,8 +34,11 @@ from .worker.kernels._deferred import enable_deferred_decode_append, flush as fl
 from .worker.kernels.paged_attn import (decode_append_and_attend, decode_rope_append_and_attend,  # noqa: F401
                                         paged_attention)
 from .worker.kernels.prefill_attn import prefill_attention, chunked_prefill_attention  # noqa: F401
-from .worker.kernels.rotary_emb import (rotary_embedding_and_store_kvcache, rotary_embedding_inplace,  # noqa: F401
-                                        rotary_tables)
+from .worker.kernels.rotary_emb import (rotary_embedding, rotary_embedding_and_store_kvcache,  # noqa: F401
+                                        rotary_embedding_inplace, rotary_scaled_tables, rotary_tables)
+from .kv8_cache import KV8Cache, allocate_kv8_cache  # noqa: F401
+from .worker.kernels.kv8 import (chunked_prefill_attention_8bit, paged_attention_8bit,  # noqa: F401
+                                 rotary_embedding_and_store_kvcache_8bit, store_kvcache_8bit)
 from .elastic_pool import ElasticKVPool  # noqa: F401
 from .kv_placement import allocate_kv_caches  # noqa: F401
 from .vmm_pool import LayerArena, VmmKVPool  # noqa: F401

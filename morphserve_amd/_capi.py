@@ -60,12 +60,52 @@ class MkvPairInfo(C.Structure):
     ]
 
 
+class MkvPool8(C.Structure):
+    """``mkv_pool8``: the 8-bit paged cache (include/morphkv.h)."""
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("num_blocks", C.c_int64),
+        ("num_layers", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("block_size", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("kind", C.c_int32),
+        ("_pad", C.c_int32),
+    ]
+
+
+class MkvBatch(C.Structure):
+    """``mkv_batch``: the rows of one step (include/morphkv.h)."""
+    _fields_ = [
+        ("block_table", C.c_void_p),
+        ("max_blocks_per_seq", C.c_int64),
+        ("table_rows", C.c_int64),
+        ("seq_ids", C.c_void_p),
+        ("prefill_start_locs", C.c_void_p),
+        ("prefill_lens", C.c_void_p),
+        ("prefix_lens", C.c_void_p),
+        ("decoding_lens", C.c_void_p),
+        ("num_prefill_seqs", C.c_int32),
+        ("num_prefill_tokens", C.c_int32),
+        ("max_prefill_len", C.c_int32),
+        ("num_decoding_seqs", C.c_int32),
+    ]
+
+
+F16, BF16 = 0, 1
+KV8_E4M3, KV8_INT8 = 0, 1
+ROPE_NONE, ROPE_HALF, ROPE_INTERLEAVED = 0, 1, 2
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
 _U64 = C.c_uint64
 _F32 = C.c_float
 _PP = C.POINTER(MkvPool)
+_PP8 = C.POINTER(MkvPool8)
+_PB = C.POINTER(MkvBatch)
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 PROTOTYPES = {
@@ -106,6 +146,13 @@ PROTOTYPES = {
     "mkv_arena_pair_grow": [_P, _P, _U64, _U64, _U64, _P, C.POINTER(MkvPairInfo)],
     "mkv_rope_store_kvcache": [_P, _P, _P, _P, _P, _PP, _P, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32,
                                _I32, _I32, _I32, _P],
+    "mkv_sizeof_pool8": [],
+    "mkv_sizeof_batch": [],
+    "mkv_store8": [_PP8, _PB, _I32, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _I64, _I64, _I32, _P, _P, _I64, _I32, _P],
+    "mkv_attn8_decode": [_PP8, _PB, _I32, _P, _P, _I64, _I64, _I32, _F32, _I32, _I32, _I32, _P, _P, _P],
+    "mkv_attn8_prefill": [_PP8, _PB, _I32, _P, _P, _I64, _I64, _I32, _F32, _I32, _I32, _I32, _P, _P, _P],
+    "mkv_rope_positions": [_I32, _I32, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I32, _I32,
+                           _I32, _I32, _P],
     "mkv_swap_blocks": [_P, _P, _I64, _I32, _PP, _P, _P, C.POINTER(_I64), _P],
     "mkv_swap_blocks_device_ids": [_P, _P, _I64, _I32, _PP, _P, _P, _I64, _P],
 }
@@ -147,6 +194,8 @@ def _load(path: str, prototypes) -> C.CDLL:
         fn.restype = _RESTYPES.get(name, C.c_int)
     if handle.mkv_sizeof_pool() != C.sizeof(MkvPool):
         raise ImportError("mkv_pool layout of the library does not match this binding")
+    if handle.mkv_sizeof_pool8() != C.sizeof(MkvPool8) or handle.mkv_sizeof_batch() != C.sizeof(MkvBatch):
+        raise ImportError("mkv_pool8 / mkv_batch layout of the library does not match this binding")
     return handle
 
 

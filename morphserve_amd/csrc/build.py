@@ -28,6 +28,10 @@ SOURCES = [
     "core.hip",
     "kv_append.hip",
     "rope.hip",
+    "rotary.hip",
+    "kv8_store.hip",
+    "attn8_decode.hip",
+    "attn8_prefill.hip",
     "paged_attn_decode.hip",
     "prefill_attn.hip",
     "block_pool.hip",
@@ -84,7 +88,7 @@ def build_library(verbose: bool = True, jobs: int = 8, diag: bool = True) -> str
     work = [(s, obj_dir, ("-DMKV_DIAG=0",)) for s in SOURCES]
     if diag:
         work += [(s, diag_dir, ("-DMKV_DIAG=1",)) for s in DIAG_SOURCES]
-    # the two attention files dominate the build: start them first
+    # the attention files dominate the build: start them first
     work.sort(key=lambda w: 0 if "attn" in w[0] else 1)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         objs = list(ex.map(lambda w: (w[1], _compile(*w)), work))

@@ -7,11 +7,16 @@ is the pair the transformer layer runs back to back
 rotated in place (prefill attention still reads the batch's own k) and the rotated k
 and v rows go straight to their cache slots, prefill and decode rows alike.
 ``rotary_tables`` builds the cos / sin cache of MorphServe/worker/model.py:230-241.
+
+``rotary_embedding`` is the rotary operator in the forms the reference lacks: half and interleaved pairs, part of the
+head, fp16 or bf16, rows of any stride, in place or into other tensors, the angles looked up by position in the fp32
+tables of ``rotary_scaled_tables`` (plain, or scaled for contexts longer than the trained one).
 """
 from __future__ import annotations
 
 import ctypes as C
-from typing import List, Tuple
+import math
+from typing import List, Optional, Tuple, Union
 
 import torch
 
@@ -77,3 +82,93 @@ def rotary_embedding_and_store_kvcache(
         _capi.ptr(st.prefill_seq_start_locs), _capi.ptr(st.prefill_seq_lens), _capi.ptr(st.decoding_seq_lens),
         st.num_prefill_seqs, st.num_prefill_tokens, st.num_decoding_seqs, q.shape[1], k.shape[1], q.shape[2],
         cur_layer, 1, _capi.current_stream()))
+
+
+def _scaled_inv_freq(rotary_dim: int, theta: float, scaling: dict, seq_len: int) -> Tuple[torch.Tensor, float]:
+    """Inverse frequencies in 64 bits and the factor of the cosines and sines, for one scaling rule."""
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    inv = theta ** (-pair / rotary_dim)
+    if kind == "default":
+        return inv, 1.0
+    factor = float(scaling["factor"])
+    if factor < 1:
+        raise ValueError(f"a rotary scaling factor is at least 1, got {factor}")
+    if kind == "linear":                                    # positions / factor
+        return inv / factor, 1.0
+    old = float(scaling.get("original_max_position_embeddings", 0))
+    if old <= 0:
+        raise ValueError(f"rotary scaling {kind!r} needs original_max_position_embeddings")
+    if kind == "dynamic":                                   # a larger base, by how far the context exceeds the trained one
+        if rotary_dim <= 2:
+            raise ValueError("rotary scaling 'dynamic' needs a rotary dim above 2")
+        grown = max(1.0, factor * max(seq_len, old) / old - (factor - 1))
+        return (theta * grown ** (rotary_dim / (rotary_dim - 2))) ** (-pair / rotary_dim), 1.0
+    if kind == "llama3":                                    # slow pairs / factor, fast pairs kept, a ramp between
+        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        if high <= low:
+            raise ValueError("high_freq_factor must exceed low_freq_factor")
+        turns = old * inv / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        return inv * keep + inv / factor * (1 - keep), 1.0
+    if kind == "yarn":                                      # the ramp runs over the pairs' numbers
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        pair_of = lambda turns: rotary_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+        first, last = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
+        ramp = ((pair / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
+        attention = scaling.get("attention_factor")
+        attention = 0.1 * math.log(factor) + 1.0 if attention is None else float(attention)
+        return inv / factor * ramp + inv * (1 - ramp), attention
+    raise ValueError(f"unknown rotary scaling {kind!r}")
+
+
+def rotary_scaled_tables(rotary_dim: int, num_positions: int, rope_theta: float = 10000.0,
+                         rope_scaling: Union[None, float, dict] = None,
+                         device: str = "cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 ``(cos, sin)`` [num_positions, rotary_dim / 2], angles computed in 64 bits (a far position times a frequency
+    loses its phase in 32).  ``rope_scaling``: ``None``, a number (linear), or the dict of a model's config with
+    ``rope_type`` one of ``default``, ``linear``, ``dynamic``, ``llama3``, ``yarn``."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if rope_scaling is None:
+        rope_scaling = {}
+    elif not isinstance(rope_scaling, dict):
+        rope_scaling = {"rope_type": "linear", "factor": float(rope_scaling)}
+    inv, mul = _scaled_inv_freq(rotary_dim, float(rope_theta), rope_scaling, num_positions)
+    angle = torch.outer(torch.arange(num_positions, dtype=torch.float64, device=device), inv.to(device))
+    return (torch.cos(angle) * mul).float(), (torch.sin(angle) * mul).float()
+
+
+def rotary_embedding(
+    q: torch.Tensor,                    # [num_tokens, num_q_heads, head_dim] fp16 or bf16
+    k: Optional[torch.Tensor],          # [num_tokens, num_kv_heads, head_dim], or None
+    positions: torch.Tensor,            # [num_tokens] int32
+    cos: torch.Tensor,                  # [max positions, rotary_dim / 2] fp32
+    sin: torch.Tensor,
+    layout: str = "half",               # pairs (d, d + rotary_dim / 2); "interleaved": pairs (2d, 2d + 1)
+    q_out: Optional[torch.Tensor] = None,         # None: in place; otherwise a tensor that does not overlap q
+    k_out: Optional[torch.Tensor] = None,
+) -> None:
+    """Rotates the first ``rotary_dim`` dims of every head by its token's position, in 32 bits, and keeps the others.  A
+    token whose position lies outside the tables gets NaN in its rotated dims."""
+    from .kv8 import DTYPES, LAYOUTS, _ints, _on, _out_rows, _require, _rows, _tables
+    _require(q.dim() == 3 and q.dtype in DTYPES, f"q must be [tokens, heads, dim] float16 or bfloat16, got {q.dtype} {tuple(q.shape)}")
+    _require(q.is_cuda, "q must be on the GPU")
+    _require(layout in LAYOUTS, f"layout must be one of {sorted(LAYOUTS)}, got {layout!r}")
+    tokens, heads, dim = q.shape
+    q_out = q if q_out is None else q_out
+    qs, qos = _rows(q, "q", q, tokens, heads, dim), _out_rows(q_out, "q_out", q, tokens, heads, dim)
+    kv_heads, ks, kos, k_ptr, k_out_ptr = 0, 0, 0, None, None
+    if k is not None:
+        _require(k.dim() == 3, f"k must be [tokens, heads, dim], got {tuple(k.shape)}")
+        k_out = k if k_out is None else k_out
+        kv_heads = k.shape[1]
+        ks, kos = _rows(k, "k", q, tokens, kv_heads, dim), _out_rows(k_out, "k_out", q, tokens, kv_heads, dim)
+        k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
+    _require(positions.dim() == 1 and positions.shape[0] == tokens, f"positions must be [{tokens}]")
+    rows, rotary_dim = _tables(cos, sin, q.device)
+    with _on(q.device):
+        _capi.check(_capi.lib().mkv_rope_positions(
+            DTYPES[q.dtype], LAYOUTS[layout], q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, qs, ks, qos, kos,
+            _ints(positions, "positions", q.device, tokens), cos.data_ptr(), sin.data_ptr(), rows, tokens, heads,
+            kv_heads, dim, rotary_dim, _capi.current_stream()))

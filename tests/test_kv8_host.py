@@ -1,0 +1,220 @@
+"""CPU checks around the 8-bit cache and the rotary forms: the oracle itself, table scaling, and that bad arguments are
+refused before anything is launched."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv8_cpu as K
+from morphserve_amd import KV8Cache, _capi, allocate_kv8_cache, rotary_embedding, rotary_scaled_tables
+from morphserve_amd.worker.kernels import kv8
+
+
+# ---- the oracle ---------------------------------------------------------------------------------------------------------
+def test_codes_round_to_nearest_even():
+    grid = K.E4M3[:127]
+    assert grid[-1] == 448 and grid[1] == 2.0 ** -9 and (np.diff(grid) > 0).all()
+    x = np.concatenate([grid, (grid[1:] + grid[:-1]) / 2, np.random.default_rng(0).uniform(0, 448, 5000)])
+    x = np.concatenate([x, -x]).astype(np.float32)
+    want = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(K.encode(x, "e4m3"), want)
+    assert np.array_equal(K.decode(K.encode(grid, "e4m3"), "e4m3"), grid)
+    assert K.encode(np.asarray([0.5, 1.5, -2.5, 127, -127, np.nan]), "int8").view(np.int8).tolist() == [0, 2, -2, 127, -127, 0]
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_exponents_and_joins(kind):
+    top = K.QMAX[kind]
+    for e in (1, 5, 120, 130):
+        edge = top * 2.0 ** (e - 127)
+        assert K.exponent(edge, kind) == e and K.exponent(np.nextafter(edge, np.inf), kind) == e + 1
+    assert K.exponent(0.0, kind) == 1
+    rng = np.random.default_rng(1)
+    slab, scale = rng.integers(0, 256, (16, 8), dtype=np.uint8), 200
+    rows = rng.standard_normal((6, 8))
+    slab, scale = K.join(slab, scale, rows[:4], 0, kind, "f16")              # a fresh block forgets its old scale
+    kept = slab.copy()
+    step = 2.0 ** (scale - 127) * (0.5 if kind == "int8" else 16)            # half a step of the largest codes
+    assert np.abs(K.decode(slab[:4], kind) * 2.0 ** (scale - 127) - rows[:4]).max() <= step
+    slab, louder = K.join(slab, scale, rows[4:] * 64, 4, kind, "f16")
+    assert louder > scale and np.array_equal(slab[6:], kept[6:])
+    step = 2.0 ** (louder - 127) * (0.5 if kind == "int8" else 16)
+    assert np.abs(K.decode(slab[:4], kind) * 2.0 ** (louder - 127) - rows[:4]).max() <= 2 * step
+    again, same = K.join(slab, louder, rows[4:] / 64, 6, kind, "f16")        # a quieter row does not lower it
+    assert same == louder and np.array_equal(again[:6], slab[:6])
+
+
+def test_attention_of_the_oracle():
+    """One block, equal keys: the mean of the values; a mask: the first value; against softmax in torch."""
+    rng = np.random.default_rng(2)
+    kc, vc = np.zeros((2, 1, 1, 16, 64), dtype=np.uint8), np.zeros((2, 1, 1, 64, 16), dtype=np.uint8)
+    scales = np.full((1, 1, 2, 2), 127, dtype=np.uint8)
+    v = rng.standard_normal((20, 1, 64))
+    table, ids = np.asarray([[1, 0]], dtype=np.int32), [0]
+    K.store(kc, vc, scales, np.zeros((20, 1, 64)), v, table, ids, [(0, 0, 0, 20)], 0, "int8", "f16")
+    _, vals, _ = K.gather(kc, vc, scales, table[0], 20, 0, 0, "int8")
+    assert np.abs(vals - v[:, 0]).max() <= 2.0 ** -6
+    q = rng.standard_normal((2, 3, 64))
+    o = K.attend(q, kc, vc, scales, table, 0, [0, 19], 0, "int8", 0.125)[0]
+    assert np.allclose(o[0], vals[0]) and np.allclose(o[1], vals.mean(0))
+    K.store(kc, vc, scales, rng.standard_normal((20, 1, 64)), v, table, ids, [(0, 0, 0, 20)], 0, "e4m3", "f16")
+    k, vals, _ = K.gather(kc, vc, scales, table[0], 20, 0, 0, "e4m3")
+    want = torch.softmax(torch.from_numpy(q[1] @ k.T * 0.125), -1).numpy() @ vals
+    assert np.allclose(K.attend(q, kc, vc, scales, table, 0, [0, 19], 0, "e4m3", 0.125)[0][1], want)
+
+
+def test_rotation_of_the_oracle():
+    x = np.random.default_rng(3).standard_normal((4, 2, 10))
+    cos, sin = (t.numpy() for t in rotary_scaled_tables(6, 9, 100.0, device="cpu"))
+    for layout in ("half", "interleaved"):
+        y = K.rotate(x, [0, 1, 5, 8], cos, sin, layout)
+        assert np.array_equal(y[0], x[0]) and np.array_equal(y[..., 6:], x[..., 6:])
+        assert np.allclose((y ** 2).sum(-1), (x ** 2).sum(-1))                              # a rotation keeps lengths
+    pair = K.rotate(np.asarray([[[1.0, 0.0]]]), [1], np.cos([[0.0], [0.3]]), np.sin([[0.0], [0.3]]), "half")[0, 0]
+    assert np.allclose(pair, [math.cos(0.3), math.sin(0.3)])
+
+
+# ---- rotary tables ------------------------------------------------------------------------------------------------------
+def test_table_scalings():
+    d, theta, n = 32, 10000.0, 64
+    inv = theta ** (-np.arange(0, d, 2) / d)
+    angle = lambda t: np.arctan2(t[1].double().numpy(), t[0].double().numpy())  # noqa: E731
+    assert np.allclose(angle(rotary_scaled_tables(d, n, theta, None, "cpu"))[1], inv, atol=1e-7)
+    for same in ({}, {"rope_type": "default"}, {"type": "default"}, 1.0):
+        assert torch.equal(rotary_scaled_tables(d, n, theta, same, "cpu")[1], rotary_scaled_tables(d, n, theta, None, "cpu")[1])
+    assert np.allclose(angle(rotary_scaled_tables(d, n, theta, 4.0, "cpu"))[1], inv / 4, atol=1e-7)
+    assert np.allclose(angle(rotary_scaled_tables(d, n, theta, {"type": "linear", "factor": 4}, "cpu"))[1], inv / 4, atol=1e-7)
+    # dynamic: untouched up to the trained length, the slowest pair slowed by the growth beyond it
+    dyn = {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 32}
+    assert np.allclose(angle(rotary_scaled_tables(d, 32, theta, dyn, "cpu"))[1], inv, atol=1e-7)
+    grown = 2.0 * 64 / 32 - 1
+    assert np.allclose(angle(rotary_scaled_tables(d, 64, theta, dyn, "cpu"))[1][[0, -1]], [inv[0], inv[-1] / grown], atol=1e-7)
+    # llama3: pairs that turn fast kept, slow ones divided
+    l3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": 256}
+    got, turns = angle(rotary_scaled_tables(d, n, theta, l3, "cpu"))[1], 256 * inv / (2 * np.pi)
+    assert np.allclose(got[turns > 4], inv[turns > 4], atol=1e-7) and np.allclose(got[turns < 1], inv[turns < 1] / 8, atol=1e-7)
+    mid = (turns > 1) & (turns < 4)
+    assert mid.any() and (got[mid] < inv[mid]).all() and (got[mid] > inv[mid] / 8).all()
+    # yarn: the same ends, and cosines scaled
+    yarn = {"rope_type": "yarn", "factor": 8.0, "original_max_position_embeddings": 1024}
+    cos, sin = rotary_scaled_tables(d, n, theta, yarn, "cpu")
+    assert cos[0, 0].item() == pytest.approx(0.1 * math.log(8) + 1)
+    got = angle((cos, sin))[1]
+    assert got[0] == pytest.approx(inv[0], abs=1e-6) and got[-1] == pytest.approx(inv[-1] / 8, rel=1e-4)
+    assert rotary_scaled_tables(d, n, theta, {**yarn, "attention_factor": 1.0}, "cpu")[0][0, 0] == 1
+
+
+@pytest.mark.parametrize("args", [(7, 4), (0, 4), (8, 4, 1e4, {"rope_type": "linear", "factor": 0.5}), (8, 4, 1e4, {"rope_type": "odd", "factor": 2, "original_max_position_embeddings": 8}),
+                                  (8, 4, 1e4, {"rope_type": "yarn", "factor": 2}), (2, 4, 1e4, {"rope_type": "dynamic", "factor": 2, "original_max_position_embeddings": 8}),
+                                  (8, 4, 1e4, {"rope_type": "llama3", "factor": 2, "low_freq_factor": 4, "high_freq_factor": 4, "original_max_position_embeddings": 8})])
+def test_table_refusals(args):
+    with pytest.raises(ValueError):
+        rotary_scaled_tables(*args, device="cpu")
+
+
+# ---- the cache object -----------------------------------------------------------------------------------------------------
+def test_cache_object():
+    cache = allocate_kv8_cache(5, (2, 3, 16, 64), torch.int8, "cpu")
+    pool = cache.descriptor()
+    assert (pool.num_blocks, pool.num_layers, pool.num_kv_heads, pool.block_size, pool.head_dim, pool.kind) == (5, 2, 3, 16, 64, 1)
+    assert pool is cache.descriptor() and pool.k == cache.k.data_ptr() and cache.num_blocks == 5
+    k, v, s = cache.k, cache.v, cache.scales
+    for bad in ((k.half(), v.half(), s), (k, v.view(torch.uint8), s), (k, k, s), (k, v, s[:1]), (k, v, s.int()),
+                (k[:, :, :, :, :32], v[:, :, :, :32], s), (k[:0], v[:0], s[:, :, :0]), (k[0], v[0], s), (k[::2], v[::2], s[:, :, ::2])):
+        with pytest.raises(ValueError):
+            KV8Cache(*bad).descriptor()
+    with pytest.raises(ValueError):
+        allocate_kv8_cache(5, (2, 3, 16, 64), torch.float16, "cpu")
+
+
+def test_split_rules():
+    for n, heads, longest in ((1, 1, 1), (1, 8, 100), (5, 8, 60000), (64, 8, 1536), (300, 32, 70), (1, 1, 10 ** 6)):
+        tps, splits = kv8.choose_split_8bit(n, heads, longest, 512)
+        assert tps % 64 == 0 and splits >= 1 and tps * splits >= longest and tps * (splits - 1) < longest
+    for seqs, hq, hkv, rows, keys in ((1, 8, 8, 1, 1), (6, 64, 8, 16, 16000), (8, 32, 32, 512, 512), (1, 1, 1, 10 ** 5, 10 ** 5)):
+        tps, splits = kv8.choose_prefill_split_8bit(seqs, hq, hkv, rows, keys, 512)
+        assert tps % 64 == 0 and splits >= 1 and tps * splits >= keys and tps * (splits - 1) < keys
+
+
+# ---- refusals of the C entries: none of these calls reaches a launch ---------------------------------------------------
+A = 1 << 20          # an address that is never followed
+
+
+def pool8(**kw):
+    p = _capi.MkvPool8(A, A, A, 10, 2, 4, 16, 128, 0, 0)
+    for name, value in kw.items():
+        setattr(p, name, value)
+    return p
+
+
+def batch8(**kw):
+    b = _capi.MkvBatch(A, 8, 4, A, A, A, A, A, 1, 5, 5, 1)
+    for name, value in kw.items():
+        setattr(b, name, value)
+    return b
+
+
+def store(p=None, b=None, dtype=0, k=A, v=A, ks=512, vs=512, layer=0, rope=0, q=A, qo=A, qs=512, qos=512, hq=4, cos=A, sin=A,
+          positions=9, rotary=32):
+    p, b = pool8() if p is None else p, batch8() if b is None else b
+    return _capi.lib().mkv_store8(C.byref(p), C.byref(b), dtype, k, v, ks, vs, layer, rope, q, qo, qs, qos, hq, cos, sin,
+                                  positions, rotary, None)
+
+
+def attn(entry, p=None, b=None, dtype=0, q=A, o=A, qs=1024, os_=1024, hq=8, layer=0, tps=64, splits=2, mid_o=A, lse=A):
+    p, b = pool8() if p is None else p, batch8() if b is None else b
+    return getattr(_capi.lib(), entry)(C.byref(p), C.byref(b), dtype, q, o, qs, os_, hq, 0.1, layer, tps, splits, mid_o, lse, None)
+
+
+BAD_POOLS = [dict(k=None), dict(v=None), dict(scales=None), dict(num_layers=0), dict(num_kv_heads=0), dict(block_size=32),
+             dict(head_dim=96), dict(kind=2), dict(num_blocks=0), dict(num_blocks=2 ** 31), dict(k=A + 8), dict(v=A + 1), dict(scales=A + 1)]
+BAD_BATCHES = [dict(block_table=None), dict(seq_ids=None), dict(max_blocks_per_seq=-1), dict(max_blocks_per_seq=2 ** 27),
+               dict(table_rows=-1), dict(num_prefill_seqs=-1), dict(num_decoding_seqs=-1), dict(max_prefill_len=-1)]
+
+
+@pytest.mark.parametrize("entry", ["store", "mkv_attn8_decode", "mkv_attn8_prefill"])
+def test_bad_pools_and_batches(entry):
+    call = store if entry == "store" else lambda **kw: attn(entry, **kw)
+    for bad in BAD_POOLS:
+        assert call(p=pool8(**bad)) == _capi.MKV_EINVAL, bad
+    for bad in BAD_BATCHES:
+        assert call(b=batch8(**bad)) == _capi.MKV_EINVAL, bad
+    assert call(dtype=2) == _capi.MKV_EINVAL and call(layer=2) == _capi.MKV_EINVAL and call(layer=-1) == _capi.MKV_EINVAL
+    lib = _capi.lib()
+    assert lib.mkv_store8(None, None, 0, A, A, 0, 0, 0, 0, None, None, 0, 0, 0, None, None, 0, 0, None) == _capi.MKV_EINVAL
+    assert call(b=batch8(num_prefill_seqs=0, num_decoding_seqs=0)) == _capi.MKV_OK          # nothing to do
+
+
+@pytest.mark.parametrize("bad", [dict(k=None), dict(v=None), dict(k=A + 8), dict(vs=516), dict(rope=3), dict(b=batch8(decoding_lens=None)),
+                                 dict(b=batch8(prefill_lens=None)), dict(rope=1, q=None), dict(rope=1, cos=None), dict(rope=1, rotary=24),
+                                 dict(rope=2, rotary=0), dict(rope=1, rotary=144), dict(rope=1, hq=0), dict(rope=1, q=A + 2),
+                                 dict(rope=1, qs=513), dict(rope=1, sin=A + 4), dict(rope=1, positions=-1), dict(rope=1, qos=1024)])
+def test_bad_store(bad):
+    assert store(**bad) == _capi.MKV_EINVAL
+    assert _capi.lib().mkv_last_error()
+
+
+@pytest.mark.parametrize("entry", ["mkv_attn8_decode", "mkv_attn8_prefill"])
+@pytest.mark.parametrize("bad", [dict(q=None), dict(o=None), dict(hq=0), dict(hq=6), dict(hq=68), dict(tps=0), dict(tps=96), dict(splits=0),
+                                 dict(mid_o=None), dict(lse=None), dict(mid_o=A + 4), dict(q=A + 2), dict(qs=1028)])
+def test_bad_attention(entry, bad):
+    assert attn(entry, **bad) == _capi.MKV_EINVAL
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=5), dict(layout=0), dict(layout=3), dict(tokens=-1), dict(hq=0), dict(hkv=-1), dict(rotary=7),
+                                 dict(rotary=0), dict(rotary=66), dict(q=None), dict(k=None), dict(pos=None), dict(cos=None),
+                                 dict(positions=-1), dict(qs=100), dict(dim=0)])
+def test_bad_rotary(bad):
+    a = dict(dtype=0, layout=1, q=A, k=A, qo=A, ko=A, qs=256, ks=128, qos=256, kos=128, pos=A, cos=A, sin=A, positions=9, tokens=3,
+             hq=4, hkv=2, dim=64, rotary=32)
+    a.update(bad)
+    assert _capi.lib().mkv_rope_positions(*[a[x] for x in ("dtype", "layout", "q", "k", "qo", "ko", "qs", "ks", "qos", "kos", "pos", "cos",
+                                                            "sin", "positions", "tokens", "hq", "hkv", "dim", "rotary")], None) == _capi.MKV_EINVAL
+
+
+def test_rows_on_the_cpu_are_refused():
+    cos, sin = rotary_scaled_tables(32, 4, device="cpu")
+    with pytest.raises(ValueError):
+        rotary_embedding(torch.zeros(2, 2, 64, dtype=torch.float16), None, torch.zeros(2, dtype=torch.int32), cos, sin)
