@@ -43,6 +43,9 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
     typedef typename T::elem E;
     typedef typename T::vec8 vec8;
     constexpr int kY = D / 64, kX = D / 32, kT = D / 16;
+    // V's scale is part of the conversion, but for int8 to bf16: there the conversion would take a product a code, and
+    // bf16's exponent has the range for a probability times a scale, 16 products a lane instead of 128
+    constexpr bool kScaleP = std::is_same<T, BF16>::value && std::is_same<C, Int8>::value;
     __shared__ float sm_acc[4][16][D];
     __shared__ float sm_m[4][16], sm_l[4][16];
 
@@ -149,7 +152,7 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
         }
 #pragma unroll
         for (int e = 0; e < 16; e += 4) l_run += (s[e] + s[e + 1]) + (s[e + 2] + s[e + 3]);
-        if constexpr (!T::kScaleV) {
+        if constexpr (kScaleP) {
             const float fv = pow2_of(ex >> 8);
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] *= fv;
@@ -165,10 +168,14 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
             const int in = min(max(valid - 4 * w, 0), 4);
             keep[w] = WHOLE || in >= 4 ? ~0u : (1u << (8 * in)) - 1u;
         }
+        auto values = [&](unsigned w0, unsigned w1) {
+            if constexpr (kScaleP) return C::raw(T{}, w0, w1);
+            else return C::scaled(T{}, w0, w1, ex >> 8);
+        };
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
-            acc[t] = T::mfma(v_operand<T, C>(x.v[t][0] & keep[0], x.v[t][1] & keep[1], ex >> 8), pb[0], acc[t]);
-            acc[t] = T::mfma(v_operand<T, C>(x.v[t][2] & keep[2], x.v[t][3] & keep[3], ex >> 8), pb[1], acc[t]);
+            acc[t] = T::mfma(values(x.v[t][0] & keep[0], x.v[t][1] & keep[1]), pb[0], acc[t]);
+            acc[t] = T::mfma(values(x.v[t][2] & keep[2], x.v[t][3] & keep[3]), pb[1], acc[t]);
         }
         after_v();
     };

@@ -1,7 +1,7 @@
 // Chunked prefill attention over the 8-bit paged cache.
 //
 // The rows of one kv head -- chunk positions times the q heads that share it, position-major -- are cut into tiles
-// of 128, one workgroup of four waves each; a wave owns two 16-row column tiles.  Keys come 64 at a time (four
+// of 64 to 256, one workgroup of four or eight waves each; a wave owns one or two 16-row column tiles.  Keys come 64 at a time (four
 // blocks): their codes are converted once, on the way into LDS, and every wave reads the converted tile from there,
 //
 //   S^T[key, row] = K . Q^T        v_mfma_f32_16x16x32
@@ -11,13 +11,21 @@
 // decode kernel the keys are numbered so that lane group c scores block c in order, which makes K's scale one factor
 // per lane and the scores, exponentiated, the operand of the second product.  V arrives transposed from the cache,
 // so that both products read LDS in rows.  Where few rows meet many keys, the keys are cut into splits.
+#include <type_traits>
+
 #include "kv8.h"
 
 namespace mkv {
 
-static constexpr int kRows = 128;             // rows per workgroup
-static constexpr int kCols = 2;               // 16-row column tiles per wave
+static constexpr int kVAhead = 4;             // V operands requested ahead of the softmax
 static constexpr float kLazyP = 8.f;
+
+// three-input maximum in one instruction (two of the two-input kind each canonicalise their operands first)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 struct Prefill8Args {
     mkv_pool8 pool;
@@ -27,29 +35,109 @@ struct Prefill8Args {
     int64_t q_stride, o_stride;               // elements
     float *mid_o, *mid_lse;
     int32_t group, layer, tiles_per_split, max_splits;
-    int32_t num_row_tiles;                    // of the longest chunk
+    int32_t sorted, key_tiles;                // row tiles by length; about the most key tiles that one sees
     float scale2;
 };
 
-// LDS rows: K has one row a key, V one a head dim.  16 bytes behind a row, and 64 more behind a block's keys, put
-// the sixteen rows that the first product's operand takes (four of each block) on different banks; V's rows of 144
-// bytes do the same for the second's.
+// LDS rows: K has one row a key, V one a head dim.  A 16-byte read of a wave is served in groups of sixteen lanes, eight
+// consecutive ones and eight of the opposite half of the next lane group, measured with feeding products: 5.1 cycles a
+// read without conflicts and 8.0 with any.  Row distances of two 16-byte slots modulo sixteen (ten serve as well),
+// eight between blocks, with the lane group one slot further, keep every such group on sixteen different slots:
+// slot 2 n + c for K and 10 n + c for V.
 template <int D>
 struct Lds8 {
-    static constexpr int kKRow = 2 * D + 16;
-    static constexpr int kKBlock = kBlk * kKRow + 64;
+    static constexpr int kKRow = 288;
+    static constexpr int kKBlock = kBlk * kKRow + 128;
     static constexpr int kK = 4 * kKBlock;
-    static constexpr int kVRow = 2 * 64 + 16;
+    static constexpr int kVRow = 160;            // keys 0 .. 7 of the four blocks, then keys 8 .. 15
     static constexpr int kV = D * kVRow;
 };
 
-template <class T, class C, int D>
-__global__ __launch_bounds__(256, 2) void attn8_prefill_kernel(const Prefill8Args g) {
+// Which row tile is the job-th longest of the batch?  A launch that does not fit the chip at once is as long as its last
+// workgroups make it, so the row tiles with most keys go first, whatever chunk they belong to.  A chunk's tiles with at
+// least t key tiles are its last ones and their number has a closed form; the t that the job falls on is found by
+// bisection, a lane counting for a chunk (or for every 64th).  False: there are not so many row tiles.
+__device__ __forceinline__ int wave_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8: sums within rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row 0's to row 1, row 2's to row 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row 1's to rows 2 and 3
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+struct ChunkTiles {
+    int rows, tiles, group, per;      // rows and row tiles of a chunk, rows per position, rows per tile
+    int prefix;
+    // row tiles that see at least t key tiles: those with a position p, prefix + p + 1 > 64 (t - 1)
+    __device__ __forceinline__ int at_least(int t) const {
+        const int64_t p = max((int64_t)64 * (t - 1) - prefix, (int64_t)0) * group;
+        return p >= rows ? 0 : tiles - (int)(p / per);
+    }
+};
+
+__device__ __forceinline__ ChunkTiles chunk_tiles(const Prefill8Args& g, int per, int b) {
+    ChunkTiles c = {0, 0, g.group, per, 0};
+    if (b < g.batch.num_prefill_seqs) {
+        c.rows = chunk_rows(chunks_of(g.batch), b, g.batch.prefill_start_locs[b]) * g.group;
+        c.tiles = (c.rows + per - 1) / per;
+        c.prefix = g.batch.prefix_lens ? max(g.batch.prefix_lens[b], 0) : 0;
+    }
+    return c;
+}
+
+__device__ __forceinline__ bool nth_longest(const Prefill8Args& g, int per, int job, int lane, int& b, int& rank) {
+    const int seqs = g.batch.num_prefill_seqs;
+    const ChunkTiles mine = chunk_tiles(g, per, lane);
+    auto count = [&](int t) {
+        int n = mine.at_least(t);
+        for (int s = lane + 64; s < seqs; s += 64) n += chunk_tiles(g, per, s).at_least(t);
+        return wave_sum(n);
+    };
+    if (job >= count(0)) return false;
+    int lo = 0, hi = g.key_tiles + 1;                         // count(lo) > job >= count(hi)
+    while (count(hi) > job) hi *= 2;                          // the host's bound may be too low
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (count(mid) > job) lo = mid;
+        else hi = mid;
+    }
+    int left = job - count(hi);                               // among the tiles with exactly lo key tiles, by chunk
+    for (int s0 = 0; s0 < seqs; s0 += 64) {
+        const ChunkTiles c = s0 ? chunk_tiles(g, per, s0 + lane) : mine;
+        const int longer = c.at_least(hi), own = c.at_least(lo) - longer;
+        int upto = own;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int x = __shfl_up(upto, s);
+            if (lane >= s) upto += x;
+        }
+        const uint64_t past = __ballot(upto > left);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            b = s0 + at;
+            rank = __shfl(longer, at) + left - (__shfl(upto, at) - __shfl(own, at));
+            b = __builtin_amdgcn_readfirstlane(b);
+            rank = __builtin_amdgcn_readfirstlane(rank);
+            return true;
+        }
+        left -= __shfl(upto, 63);
+    }
+    return false;
+}
+
+template <class T, class C, int D, int WAVES, int COLS>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn8_prefill_kernel(const Prefill8Args g) {
     typedef typename T::elem E;
     typedef typename T::vec8 vec8;
     typedef E vec4 __attribute__((ext_vector_type(4)));
     typedef Lds8<D> L;
-    constexpr int kX = D / 32, kT = D / 16, kU = D / 64;      // steps, dim tiles, 16-byte units a thread stages
+    constexpr int kThreads = 64 * WAVES;
+    constexpr int kRows = 16 * COLS * WAVES;                 // rows per workgroup
+    constexpr int kX = D / 32, kT = D / 16;                   // steps of the first product, dim tiles of the second
+    constexpr int kUnits = 4 * D;                             // 16-byte units of a tile's K (and V) slabs
+    constexpr int kU = kUnits >= kThreads ? kUnits / kThreads : 1;
     __shared__ __attribute__((aligned(16))) char k_lds[2][L::kK];
     __shared__ __attribute__((aligned(16))) char v_lds[2][L::kV];
 
@@ -58,22 +146,22 @@ __global__ __launch_bounds__(256, 2) void attn8_prefill_kernel(const Prefill8Arg
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15;
     const int c = lane >> 4;
-    // Consecutive workgroups go to the eight XCDs in turn: the low three bits pick the (sequence, kv head) residue,
-    // so that all row tiles and splits of a pair share one L2.  Row tiles with most keys come first.
+    // Workgroups are numbered (row tile, split, kv head), the head fastest: consecutive ones go to the eight XCDs in
+    // turn, so that with eight kv heads or a multiple a head's row tiles share one L2.
     const int Hkv = g.pool.num_kv_heads;
-    const int pairs = Hkv * g.batch.num_prefill_seqs;
-    const int pairs_x = (pairs + 7) >> 3;
-    const int slot = (int)(blockIdx.x >> 3);
-    const int job = slot / pairs_x;
-    const int pair = (slot - job * pairs_x) * 8 + (int)(blockIdx.x & 7);
-    if (pair >= pairs) return;
-    const int rank = job / g.max_splits;
-    const int split = job - rank * g.max_splits;
-    const int kvh = pair % Hkv;
-    const int b = pair / Hkv;
-
     const int G = g.group;
     const int Hq = Hkv * G;
+    const int cell = (int)(blockIdx.x / (unsigned)Hkv);
+    const int kvh = (int)blockIdx.x - cell * Hkv;
+    const int job = cell / g.max_splits;
+    const int split = cell - job * g.max_splits;
+    int b, rank;                                              // rank: the row tile, counted from the chunk's last
+    if (g.sorted) {
+        if (!nth_longest(g, kRows, job, lane, b, rank)) return;
+    } else {
+        rank = job / g.batch.num_prefill_seqs;
+        b = job - rank * g.batch.num_prefill_seqs;
+    }
     const int64_t start = g.batch.prefill_start_locs[b];
     const int len = chunk_rows(chunks_of(g.batch), b, start);
     const int rows = len * G;
@@ -94,11 +182,11 @@ __global__ __launch_bounds__(256, 2) void attn8_prefill_kernel(const Prefill8Arg
     const int num_blocks = (int)g.pool.num_blocks;
 
     // this wave's rows and Q^T: lane (row n, group c) holds dims 32 x + 8 c .. + 8 for step x
-    const int r0 = row0 + wave * 16 * kCols;
-    vec8 qb[kCols][kX];
-    int last_key[kCols];                                      // a row sees keys 0 .. its own position
+    const int r0 = row0 + wave * 16 * COLS;
+    vec8 qb[COLS][kX];
+    int last_key[COLS];                                      // a row sees keys 0 .. its own position
 #pragma unroll
-    for (int u = 0; u < kCols; ++u) {
+    for (int u = 0; u < COLS; ++u) {
         const int r = r0 + 16 * u + n;
         const int t = r / G;
         const E* qrow = (const E*)g.q + (start + t) * g.q_stride + ((int64_t)kvh * G + (r - t * G)) * D;
@@ -109,15 +197,17 @@ __global__ __launch_bounds__(256, 2) void attn8_prefill_kernel(const Prefill8Arg
             else qb[u][x] = (vec8)(E)0.f;
         }
     }
-    const int wave_first = r0 < rows ? (int)min(prefix + r0 / G, room - 1) : -1;                      // first row's last key
-    const int wave_last = r0 < rows ? (int)min(prefix + (min(r0 + 16 * kCols, rows) - 1) / G, room - 1) : -1;
+    const int wave_last = r0 < rows ? (int)min(prefix + (min(r0 + 16 * COLS, rows) - 1) / G, room - 1) : -1;
 
-    float4v acc[kCols][kT];
-    float m_run[kCols], l_run[kCols];
+    // Row sums come out of the matrix cores too: a V^T row of ones makes every register of lsum the row's sum of
+    // the rounded probabilities, the ones the numerator is built from.
+    float4v acc[COLS][kT], lsum[COLS];
+    float m_run[COLS];
+    const vec8 ones = (vec8)(E)1.f;
 #pragma unroll
-    for (int u = 0; u < kCols; ++u) {
+    for (int u = 0; u < COLS; ++u) {
         m_run[u] = kFar;
-        l_run[u] = 0.f;
+        lsum[u] = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < kT; ++t) acc[u][t] = (float4v){0.f, 0.f, 0.f, 0.f};
     }
@@ -128,145 +218,188 @@ __global__ __launch_bounds__(256, 2) void attn8_prefill_kernel(const Prefill8Arg
     const uint8_t* v_base = (const uint8_t*)g.pool.v + slab;
     const uint16_t* scales = scale_row8(g.pool, g.layer, kvh);
 
-    // ---- staging: a tile's slabs are 4 D units of 16 bytes each for K and V; unit w belongs to block w / D ----------
+    // ---- staging: unit w of a tile's slabs belongs to block w / D; a thread takes units tid, tid + kThreads, ... ---------
     auto id_of = [&](int blk) {
         const int pid = blk < nblk ? table[blk] : -1;
         return pid >= 0 && pid < num_blocks ? pid : -1;
     };
+    const bool stages = tid < kUnits;                         // the same for a wave
     uint4v kreg[kU], vreg[kU];
-    unsigned ereg[kU];                                        // exponents of the staged units' blocks
-    int st_pid[kU];                                           // their ids, one tile ahead
-    int my_pid, my_pid_next;                                  // ids of block c of the current / staged tile
-    unsigned my_ex, my_ex_next;
+    int valid[kU];                                            // keys of the units' blocks that count
+    unsigned ereg[kU];                                        // the blocks' exponents
+    int ids[kU], id_c;                                        // of the tile after the fetched one: units' blocks, block c
+    bool here = false, here_next = false;                     // block c of the current / fetched tile
+    unsigned ex = 0, ex_next = 0;
     auto load_ids = [&](int tile) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) st_pid[u] = id_of(4 * tile + (tid + 256 * u) / D);
-        my_pid_next = id_of(4 * tile + c);
+        for (int u = 0; u < kU; ++u) ids[u] = id_of(4 * tile + (tid + kThreads * u) / D);
+        id_c = id_of(4 * tile + c);
     };
-    auto fetch = [&]() {
+    // requests the codes of `tile` and the ids of the one after it
+    auto fetch = [&](int tile) {
+        if (stages) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int64_t at = (int64_t)max(st_pid[u], 0) * block_bytes + 16 * ((tid + 256 * u) % D);
-            kreg[u] = *(const uint4v*)(k_base + at);
-            vreg[u] = *(const uint4v*)(v_base + at);
-            ereg[u] = st_pid[u] >= 0 ? scales[st_pid[u]] : 0x7f7fu;
+            for (int u = 0; u < kU; ++u) {
+                const int64_t at = (int64_t)max(ids[u], 0) * block_bytes + 16 * ((tid + kThreads * u) % D);
+                kreg[u] = *(const uint4v*)(k_base + at);
+                vreg[u] = *(const uint4v*)(v_base + at);
+                ereg[u] = scales[max(ids[u], 0)];
+                valid[u] = ids[u] >= 0 ? min(max(kv_len - (4 * tile + (tid + kThreads * u) / D) * kBlk, 0), kBlk) : 0;
+            }
         }
-        my_ex_next = my_pid_next >= 0 ? scales[my_pid_next] : 0x7f7fu;
+        ex_next = scales[max(id_c, 0)];
+        here_next = id_c >= 0;
+        load_ids(tile + 1);                                   // past the end: no block
     };
-    auto stage = [&](int buf, int tile) {
+    auto stage = [&](int buf) {
+        if (!stages) return;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int w = tid + 256 * u;
+            const int w = tid + kThreads * u;
             const int blk = w / D, o = w % D;
-            // K: 16 dims of a key
+            // K: 16 dims of a key; a block that is not there is one of zeros
+            const unsigned there = valid[u] > 0 ? ~0u : 0u;
             char* kd = k_lds[buf] + blk * L::kKBlock + (o * 16 / D) * L::kKRow + (o * 16 % D) * 2;
-            *(vec8*)kd = C::raw(T{}, kreg[u][0], kreg[u][1]);
-            *(vec8*)(kd + 16) = C::raw(T{}, kreg[u][2], kreg[u][3]);
-            // V: 16 keys of a dim; codes behind the last key, and of a block that is not there, count as 0
-            const int valid = st_pid[u] >= 0 ? min(max(kv_len - (4 * tile + blk) * kBlk, 0), kBlk) : 0;
+            *(vec8*)kd = C::raw(T{}, kreg[u][0] & there, kreg[u][1] & there);
+            *(vec8*)(kd + 16) = C::raw(T{}, kreg[u][2] & there, kreg[u][3] & there);
+            // V: 16 keys of a dim; codes behind the last key count as 0
             unsigned keep[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int in = min(max(valid - 4 * j, 0), 4);
+                const int in = min(max(valid[u] - 4 * j, 0), 4);
                 keep[j] = in >= 4 ? ~0u : (1u << (8 * in)) - 1u;
             }
-            char* vd = v_lds[buf] + o * L::kVRow + blk * 32;
-            *(vec8*)vd = v_operand<T, C>(vreg[u][0] & keep[0], vreg[u][1] & keep[1], ereg[u] >> 8);
-            *(vec8*)(vd + 16) = v_operand<T, C>(vreg[u][2] & keep[2], vreg[u][3] & keep[3], ereg[u] >> 8);
+            const unsigned ev = valid[u] > 0 ? ereg[u] >> 8 : 127u;
+            char* vd = v_lds[buf] + o * L::kVRow + blk * 16;
+            *(vec8*)vd = C::scaled(T{}, vreg[u][0] & keep[0], vreg[u][1] & keep[1], ev);
+            *(vec8*)(vd + 64) = C::scaled(T{}, vreg[u][2] & keep[2], vreg[u][3] & keep[3], ev);
         }
     };
 
     const int k_rd = (n >> 2) * L::kKBlock + (n & 3) * L::kKRow + 16 * c;      // + 4 j rows, + 64 x bytes
-    const int v_rd = n * L::kVRow + 32 * c;                                    // + 16 t rows, + 16 z bytes
+    const int v_rd = n * L::kVRow + 16 * c;                                    // + 16 t rows, + 64 z bytes
 
-    auto consume = [&](int buf, int tile) {
-        const bool here = my_pid >= 0;
-        const bool careful = __ballot(!here) != 0 || tile * 64 + 63 > wave_first;      // the same for the wave
-        const float f = g.scale2 * pow2_of(my_ex & 0xffu);
-        const int key0 = (4 * tile + c) * kBlk;
-        float4v st[kCols][4];
+    // One tile against the wave's rows.  MASKED: a row may not see all of its keys.
+    auto consume = [&](auto masked_tag, int buf, int tile) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
+        const char* kl = k_lds[buf] + k_rd;
+        const char* vl = v_lds[buf] + v_rd;
+        // the matrix phases run at raised priority: the SIMD's other wave fills the gaps with its softmax.  K operands of
+        // the next score tile are requested ahead of the products of this one.
+        __builtin_amdgcn_s_setprio(2);
+        float4v st[COLS][4];
+        vec8 ka[2][kX];
+#pragma unroll
+        for (int x = 0; x < kX; ++x) ka[0][x] = *(const vec8*)(kl + 64 * x);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (j < 3) {
 #pragma unroll
-            for (int u = 0; u < kCols; ++u) st[u][j] = (float4v){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int x = 0; x < kX; ++x) {
-                const vec8 ka = *(const vec8*)(k_lds[buf] + k_rd + 4 * j * L::kKRow + 64 * x);
-#pragma unroll
-                for (int u = 0; u < kCols; ++u) st[u][j] = T::mfma(ka, qb[u][x], st[u][j]);
+                for (int x = 0; x < kX; ++x) ka[(j + 1) & 1][x] = *(const vec8*)(kl + 4 * (j + 1) * L::kKRow + 64 * x);
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < COLS; ++u) st[u][j] = (float4v){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < kX; ++x)
+#pragma unroll
+                for (int u = 0; u < COLS; ++u) st[u][j] = T::mfma(ka[j & 1][x], qb[u][x], st[u][j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        vec8 pb[kCols][2];
+        // V operands of the first dim tiles are requested before the softmax, which covers their way
+        vec8 va[kVAhead];
 #pragma unroll
-        for (int u = 0; u < kCols; ++u) {
-            float s[16], mx = kFar;
+        for (int e = 0; e < kVAhead; ++e) va[e] = *(const vec8*)(vl + 16 * (e >> 1) * L::kVRow + 64 * (e & 1));
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
+        const float f = g.scale2 * pow2_of(here ? ex & 0xffu : 127u);    // > 0: keeps the order of the scores
+        vec8 pb[COLS][2];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[e] = st[u][e >> 2][e & 3] * f;
-                if (careful && !(here && key0 + e <= last_key[u])) s[e] = kFar;
-                mx = fmaxf(mx, s[e]);
+        for (int u = 0; u < COLS; ++u) {
+            const int seen = MASKED ? (here ? last_key[u] - (4 * tile + c) * kBlk + 1 : 0) : kBlk;   // of the lane's sixteen keys
+            float s[16], mx;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = st[u][e >> 2][e & 3];
+            if (MASKED) {
+                mx = kFar;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[e] = e < seen ? s[e] * f : kFar;
+                    mx = fmaxf(mx, s[e]);
+                }
+            } else {
+                mx = max3(max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[8])),
+                          max3(s[9], s[10], s[11]), max3(max3(s[12], s[13], s[14]), s[15], s[15])) * f;
+                mx = here ? mx : kFar;
             }
             if (__ballot(mx - m_run[u] > kLazyP) != 0) {
                 const float m_new = fmaxf(m_run[u], max_over_quarters(mx));
                 const float alpha = __builtin_amdgcn_exp2f(m_run[u] - m_new);
-                l_run[u] *= alpha;
+                lsum[u] *= alpha;
 #pragma unroll
                 for (int t = 0; t < kT; ++t) acc[u][t] *= alpha;
                 m_run[u] = m_new;
             }
+            const float off = here ? -m_run[u] : kFar;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] - m_run[u]);
-                if (careful && !(here && key0 + e <= last_key[u])) s[e] = 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) l_run[u] += (s[e] + s[e + 1]) + (s[e + 2] + s[e + 3]);
-            if constexpr (!T::kScaleV) {
-                const float fv = pow2_of(my_ex >> 8);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] *= fv;
+                if (MASKED) s[e] = e < seen ? __builtin_amdgcn_exp2f(s[e] - m_run[u]) : 0.f;
+                else s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f, off));
             }
 #pragma unroll
             for (int z = 0; z < 2; ++z)
                 pb[u][z] = (vec8){(E)s[8 * z], (E)s[8 * z + 1], (E)s[8 * z + 2], (E)s[8 * z + 3],
                                   (E)s[8 * z + 4], (E)s[8 * z + 5], (E)s[8 * z + 6], (E)s[8 * z + 7]};
         }
+        __builtin_amdgcn_s_setprio(2);
+#pragma unroll
+        for (int u = 0; u < COLS; ++u) {
+            lsum[u] = T::mfma(ones, pb[u][0], lsum[u]);
+            lsum[u] = T::mfma(ones, pb[u][1], lsum[u]);
+        }
 #pragma unroll
         for (int t = 0; t < kT; ++t)
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-                const vec8 va = *(const vec8*)(v_lds[buf] + v_rd + 16 * t * L::kVRow + 16 * z);
+                const int e = 2 * t + z;
+                const vec8 a = e < kVAhead ? va[e % kVAhead] : *(const vec8*)(vl + 16 * t * L::kVRow + 64 * z);
 #pragma unroll
-                for (int u = 0; u < kCols; ++u) acc[u][t] = T::mfma(va, pb[u][z], acc[u][t]);
+                for (int u = 0; u < COLS; ++u) acc[u][t] = T::mfma(a, pb[u][z], acc[u][t]);
             }
+        __builtin_amdgcn_s_setprio(0);
     };
 
     if (tile_begin < tile_end) {
         load_ids(tile_begin);
-        fetch();
-        stage(0, tile_begin);
-        my_pid = my_pid_next;
-        my_ex = my_ex_next;
-        load_ids(tile_begin + 1);                             // past the end: no block
+        fetch(tile_begin);
+        stage(0);
+        here = here_next;
+        ex = ex_next;
     }
-    for (int tile = tile_begin; tile < tile_end; ++tile) {
-        const int buf = (tile - tile_begin) & 1;
-        const bool more = tile + 1 < tile_end;
-        __syncthreads();                                      // this tile is staged; the other buffer is free
-        if (more) fetch();
-        if (tile * 64 <= wave_last) consume(buf, tile);
-        if (more) {
-            stage(buf ^ 1, tile + 1);
-            my_pid = my_pid_next;
-            my_ex = my_ex_next;
-            load_ids(tile + 2);
+    auto iterate = [&](auto masked_tag, int from, int to) {
+        for (int tile = from; tile < to; ++tile) {
+            const int buf = (tile - tile_begin) & 1;
+            const bool more = tile + 1 < tile_end;
+            __syncthreads();                                  // this tile is staged; the other buffer is free
+            if (more) fetch(tile + 1);
+            if (tile * 64 <= wave_last) consume(masked_tag, buf, tile);
+            if (more) {
+                stage(buf ^ 1);
+                here = here_next;
+                ex = ex_next;
+            }
         }
-    }
+    };
+    // The tiles that every row of the workgroup sees whole, then those that hold some row's last key.  Two loops, not two
+    // bodies in one: the accumulators would be copied where the bodies meet, and the registers do not suffice for that.
+    const int full_end = max(tile_begin, min(tile_end, (int)((min(prefix + row0 / G, room - 1) + 1) >> 6)));
+    iterate(std::false_type{}, tile_begin, full_end);
+    iterate(std::true_type{}, full_end, tile_end);
 
     // ---- output: a lane holds, of row n of a column tile, dims 16 t + 4 c .. + 4 -------------------------------------
 #pragma unroll
-    for (int u = 0; u < kCols; ++u) {
-        const float l = sum_over_quarters(l_run[u]);
+    for (int u = 0; u < COLS; ++u) {
+        const float l = lsum[u][0];
         const int r = r0 + 16 * u + n;
         if (r >= rows) continue;
         const float inv = l == 0.f ? 0.f : 1.f / l;           // a row with nothing to attend to: zeros
@@ -287,10 +420,19 @@ __global__ __launch_bounds__(256, 2) void attn8_prefill_kernel(const Prefill8Arg
     }
 }
 
-template <class T, class C>
-static void launch_prefill8(int head_dim, dim3 grid, hipStream_t s, const Prefill8Args& g) {
-    if (head_dim == 128) hipLaunchKernelGGL((attn8_prefill_kernel<T, C, 128>), grid, dim3(256), 0, s, g);
-    else hipLaunchKernelGGL((attn8_prefill_kernel<T, C, 64>), grid, dim3(256), 0, s, g);
+template <class T, class C, int D>
+static void launch_prefill8(int shape, dim3 grid, hipStream_t s, const Prefill8Args& g) {
+    if (shape == 256) hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 8, 2>), grid, dim3(512), 0, s, g);
+    else if (shape == 128) hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 4, 2>), grid, dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 4, 1>), grid, dim3(256), 0, s, g);
+}
+
+template <class T>
+static void launch_prefill8(const mkv_pool8& p, int shape, dim3 grid, hipStream_t s, const Prefill8Args& g) {
+    if (p.kind == MKV_KV8_E4M3 && p.head_dim == 128) launch_prefill8<T, E4M3, 128>(shape, grid, s, g);
+    else if (p.kind == MKV_KV8_E4M3) launch_prefill8<T, E4M3, 64>(shape, grid, s, g);
+    else if (p.head_dim == 128) launch_prefill8<T, Int8, 128>(shape, grid, s, g);
+    else launch_prefill8<T, Int8, 64>(shape, grid, s, g);
 }
 
 }  // namespace mkv
@@ -315,6 +457,7 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     MKV_REQUIRE(max_splits == 1 || (mid_o && mid_lse), "scratch buffers are NULL");
     MKV_REQUIRE(((uintptr_t)mid_o & 15) == 0 && ((uintptr_t)mid_lse & 3) == 0, "mid_o must be 16-byte aligned, mid_lse 4-byte aligned");
     MKV_REQUIRE((((uintptr_t)q | (uintptr_t)o) & 15) == 0 && ((q_stride | o_stride) & 7) == 0, "q and o rows must be 16-byte aligned");
+    MKV_REQUIRE(softmax_scale > 0.f, "softmax_scale must be positive");
     const int group = num_q_heads / pool->num_kv_heads;
     MKV_REQUIRE((int64_t)batch->max_prefill_len * num_q_heads <= 0x7fffff00 && batch->num_prefill_seqs <= 65535,
                 "too many rows in one call");
@@ -331,20 +474,23 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     g.layer = layer;
     g.tiles_per_split = tokens_per_split / 64;
     g.max_splits = max_splits;
-    g.num_row_tiles = mkv::cdiv((int64_t)batch->max_prefill_len * group, mkv::kRows);
     g.scale2 = softmax_scale * mkv::kLog2E;
-    const int64_t pairs_x = ((int64_t)pool->num_kv_heads * batch->num_prefill_seqs + 7) / 8;
-    const int64_t cells = pairs_x * 8 * g.num_row_tiles * max_splits;
+    const int64_t rows = (int64_t)batch->max_prefill_len * group;
+    const int64_t columns = (int64_t)pool->num_kv_heads * max_splits * batch->num_prefill_seqs;
+    // Rows per workgroup: 64 where a chunk has no more; 256 (one workgroup of eight waves per CU, the conversions of a
+    // tile shared by more rows) for long chunks that fill the chip with them -- 2048 x 4 rows over 8192 cached tokens
+    // 425 us against 433 with 128 (int8, bf16: 434 against 464), but 512 rows 53 against 48.
+    const int shape = rows <= 64 ? 64 : rows > 512 && columns * mkv::cdiv(rows, 256) >= mkv::num_cus() ? 256 : 128;
+    const int64_t cells = columns * mkv::cdiv(rows, shape);
     MKV_REQUIRE(cells <= 0x7fffffff, "too many rows in one call");
+    // Finding a workgroup's place in the order costs a few microseconds: 8 x 512 tokens 48 us, sorted 52; four ragged
+    // chunks over up to 7473 cached tokens 1211 us, sorted 676.
+    g.key_tiles = mkv::cdiv((int64_t)tokens_per_split * max_splits, 64);
+    g.sorted = batch->num_prefill_seqs > 1 && cells > 2 * mkv::num_cus() && g.key_tiles >= 32;
     const dim3 grid((unsigned)cells);
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == MKV_F16) {
-        if (pool->kind == MKV_KV8_E4M3) mkv::launch_prefill8<mkv::F16, mkv::E4M3>(pool->head_dim, grid, s, g);
-        else mkv::launch_prefill8<mkv::F16, mkv::Int8>(pool->head_dim, grid, s, g);
-    } else {
-        if (pool->kind == MKV_KV8_E4M3) mkv::launch_prefill8<mkv::BF16, mkv::E4M3>(pool->head_dim, grid, s, g);
-        else mkv::launch_prefill8<mkv::BF16, mkv::Int8>(pool->head_dim, grid, s, g);
-    }
+    if (dtype == MKV_F16) mkv::launch_prefill8<mkv::F16>(*pool, shape, grid, s, g);
+    else mkv::launch_prefill8<mkv::BF16>(*pool, shape, grid, s, g);
     MKV_HIP(hipGetLastError());
     if (max_splits > 1)
         return mkv::launch_merge8(dtype, pool->head_dim, (const float*)mid_o, (const float*)mid_lse, o, o_stride,

@@ -6,8 +6,8 @@
 //
 // A code stands for code * 2^(scale - 127).  Scales are powers of two, so that applying one is exact: a code's
 // value is an fp16 / bf16 number, e4m3 codes change their scale without another rounding (but for codes that fall
-// among its subnormals), and every kernel may apply the scale where that is cheapest -- K's to the scores, V's in
-// the conversion (fp16) or to the probabilities (bf16, whose exponent has the range).  Within a block V lies
+// among its subnormals), and every kernel may apply the scale where that is cheapest: K's to the scores, V's in the
+// conversion or to the probabilities.  Within a block V lies
 // transposed because that is the operand order of the second product: a lane's 16 bytes are the 16 tokens
 // of one head dim, and no transpose stands between memory and the matrix cores.  The scales lie apart from the
 // codes, by layer and head: a layer's attention reads one dense array, not one byte out of every cache line.
@@ -34,7 +34,6 @@ struct F16 {
     typedef half8 vec8;
     // rows are clamped to the largest value whose code cannot stand for an infinity of the type
     static constexpr float kMost = 61440.f;       // 1.875 * 2^15
-    static constexpr bool kScaleV = true;         // V's scale is applied to V: probabilities times a scale would leave fp16's range
     static __device__ __forceinline__ float4v mfma(vec8 a, vec8 b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -43,7 +42,6 @@ struct BF16 {
     typedef __bf16 elem;
     typedef bf8 vec8;
     static constexpr float kMost = 0x1.ep127f;    // 1.875 * 2^127
-    static constexpr bool kScaleV = false;        // V's scale goes to the probabilities: 16 products a lane instead of 128
     static __device__ __forceinline__ float4v mfma(vec8 a, vec8 b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -78,14 +76,16 @@ struct E4M3 {
         const half2v d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, s, true);
         return (half8){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
     }
-    static __device__ __forceinline__ half8 raw(F16 t, unsigned w0, unsigned w1) { return scaled(t, w0, w1, 127u); }
-    static __device__ __forceinline__ bf8 raw(BF16, unsigned w0, unsigned w1) {
-        const bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, false);
-        const bf2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, true);
-        const bf2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, false);
-        const bf2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, true);
+    static __device__ __forceinline__ bf8 scaled(BF16, unsigned w0, unsigned w1, unsigned e) {
+        const float s = pow2_of(e);
+        const bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false);
+        const bf2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true);
+        const bf2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false);
+        const bf2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
         return (bf8){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
     }
+    template <class T>
+    static __device__ __forceinline__ typename T::vec8 raw(T t, unsigned w0, unsigned w1) { return scaled(t, w0, w1, 127u); }
 };
 
 struct Int8 {
@@ -124,6 +124,19 @@ struct Int8 {
         const _Float16 f1 = __builtin_bit_cast(_Float16, (unsigned short)((x1 + 15) << 10));
         return raw(t, w0, w1) * f0 * f1;
     }
+    static __device__ __forceinline__ bf8 scaled(BF16, unsigned w0, unsigned w1, unsigned e) {
+        const float s = pow2_of(e);
+        float a[4], b[4];
+        decode4(w0, a);
+        decode4(w1, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] *= s;
+            b[j] *= s;
+        }
+        return (bf8){(__bf16)a[0], (__bf16)a[1], (__bf16)a[2], (__bf16)a[3],
+                     (__bf16)b[0], (__bf16)b[1], (__bf16)b[2], (__bf16)b[3]};
+    }
     static __device__ __forceinline__ bf8 raw(BF16, unsigned w0, unsigned w1) {
         float a[4], b[4];
         decode4(w0, a);
@@ -132,13 +145,6 @@ struct Int8 {
                      (__bf16)b[0], (__bf16)b[1], (__bf16)b[2], (__bf16)b[3]};
     }
 };
-
-// V codes to the operand: with their scale where the type wants it there
-template <class T, class C>
-__device__ __forceinline__ typename T::vec8 v_operand(unsigned w0, unsigned w1, unsigned e) {
-    if constexpr (T::kScaleV) return C::scaled(T{}, w0, w1, e);
-    else return C::raw(T{}, w0, w1);
-}
 
 // Bytes of one block in either code tensor, and of one (layer, head) slab in it.
 __host__ __device__ __forceinline__ int64_t block_bytes8(const mkv_pool8& p) {

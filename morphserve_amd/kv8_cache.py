@@ -37,25 +37,27 @@ class KV8Cache:
         return self.k.shape[0]
 
     def descriptor(self) -> _capi.MkvPool8:
-        """The cache as the C entries take it; the tensors are checked the first time and must not be exchanged
-        afterwards (make another ``KV8Cache`` for other tensors)."""
+        """The cache as the C entries take it.  The tensors are checked the first time and must not be exchanged
+        afterwards: make another ``KV8Cache`` for other tensors."""
         if self._pool is None:
             k, v, scales = self.k, self.v, self.scales
-            if k.dtype not in KINDS or v.dtype != k.dtype:
-                raise ValueError(f"an 8-bit cache holds float8_e4m3fn or int8 codes, got {k.dtype} / {v.dtype}")
-            if k.dim() != 5 or k.numel() == 0:
-                raise ValueError(f"k must be [num_blocks, L, Hkv, block_size, D], got {tuple(k.shape)}")
-            n, layers, heads, block, dim = k.shape
-            if tuple(v.shape) != (n, layers, heads, dim, block):
+            dtype, shape, device = k.dtype, k.shape, k.device
+            if dtype not in KINDS or v.dtype != dtype:
+                raise ValueError(f"an 8-bit cache holds float8_e4m3fn or int8 codes, got {dtype} / {v.dtype}")
+            if len(shape) != 5 or 0 in shape:
+                raise ValueError(f"k must be [num_blocks, L, Hkv, block_size, D], got {tuple(shape)}")
+            n, layers, heads, block, dim = shape
+            if v.shape != (n, layers, heads, dim, block):
                 raise ValueError(f"v must be {(n, layers, heads, dim, block)}, got {tuple(v.shape)}")
-            if scales.dtype != torch.uint8 or tuple(scales.shape) != (layers, heads, n, 2):
+            if scales.dtype != torch.uint8 or scales.shape != (layers, heads, n, 2):
                 raise ValueError(f"scales must be uint8 {(layers, heads, n, 2)}, got {scales.dtype} {tuple(scales.shape)}")
             if not (k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
                 raise ValueError("the tensors of an 8-bit cache must be contiguous")
-            if not (k.device == v.device == scales.device):
+            if v.device != device or scales.device != device:
                 raise ValueError("the tensors of an 8-bit cache must be on one device")
+            self.shape, self.device = tuple(shape), device
             self._pool = _capi.MkvPool8(k.data_ptr(), v.data_ptr(), scales.data_ptr(), n, layers, heads, block, dim,
-                                        KINDS[k.dtype], 0)
+                                        KINDS[dtype], 0)
         return self._pool
 
 

@@ -151,24 +151,27 @@ def rotary_embedding(
 ) -> None:
     """Rotates the first ``rotary_dim`` dims of every head by its token's position, in 32 bits, and keeps the others.  A
     token whose position lies outside the tables gets NaN in its rotated dims."""
-    from .kv8 import DTYPES, LAYOUTS, _ints, _on, _out_rows, _require, _rows, _tables
-    _require(q.dim() == 3 and q.dtype in DTYPES, f"q must be [tokens, heads, dim] float16 or bfloat16, got {q.dtype} {tuple(q.shape)}")
-    _require(q.is_cuda, "q must be on the GPU")
-    _require(layout in LAYOUTS, f"layout must be one of {sorted(LAYOUTS)}, got {layout!r}")
+    from .kv8 import DTYPES, _ints, _layout, _on, _out_rows, _rows, _stream, _tables
+    dtype, dev = q.dtype, q.device
+    if q.dim() != 3 or dtype not in DTYPES or dev.type != "cuda":
+        raise ValueError(f"q must be [tokens, heads, dim] float16 or bfloat16 on the GPU, got {dtype} {tuple(q.shape)} on {dev}")
+    rope = _layout(layout)
     tokens, heads, dim = q.shape
     q_out = q if q_out is None else q_out
-    qs, qos = _rows(q, "q", q, tokens, heads, dim), _out_rows(q_out, "q_out", q, tokens, heads, dim)
+    qs, qos = _rows(q, "q", dtype, dev, tokens, heads, dim), _out_rows(q_out, "q_out", dtype, dev, tokens, heads, dim)
     kv_heads, ks, kos, k_ptr, k_out_ptr = 0, 0, 0, None, None
     if k is not None:
-        _require(k.dim() == 3, f"k must be [tokens, heads, dim], got {tuple(k.shape)}")
+        if k.dim() != 3:
+            raise ValueError(f"k must be [tokens, heads, dim], got {tuple(k.shape)}")
         k_out = k if k_out is None else k_out
         kv_heads = k.shape[1]
-        ks, kos = _rows(k, "k", q, tokens, kv_heads, dim), _out_rows(k_out, "k_out", q, tokens, kv_heads, dim)
+        ks, kos = _rows(k, "k", dtype, dev, tokens, kv_heads, dim), _out_rows(k_out, "k_out", dtype, dev, tokens, kv_heads, dim)
         k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
-    _require(positions.dim() == 1 and positions.shape[0] == tokens, f"positions must be [{tokens}]")
-    rows, rotary_dim = _tables(cos, sin, q.device)
-    with _on(q.device):
+    if positions.shape != (tokens,):
+        raise ValueError(f"positions must be [{tokens}], got {tuple(positions.shape)}")
+    pos = _ints(positions, "positions", dev, tokens)
+    rows, rotary_dim = _tables(cos, sin, dev)
+    with _on(dev):
         _capi.check(_capi.lib().mkv_rope_positions(
-            DTYPES[q.dtype], LAYOUTS[layout], q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, qs, ks, qos, kos,
-            _ints(positions, "positions", q.device, tokens), cos.data_ptr(), sin.data_ptr(), rows, tokens, heads,
-            kv_heads, dim, rotary_dim, _capi.current_stream()))
+            DTYPES[dtype], rope, q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, qs, ks, qos, kos, pos, cos.data_ptr(),
+            sin.data_ptr(), rows, tokens, heads, kv_heads, dim, rotary_dim, _stream(dev)))

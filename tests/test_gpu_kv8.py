@@ -287,6 +287,19 @@ def test_chunks_split_over_the_keys(cuda, monkeypatch, dtype, kind, splits):
     assert_within(prefill(b, cuda, q), *b.expect_chunks(q))
 
 
+@pytest.mark.parametrize("hint", [True, False])
+@pytest.mark.parametrize("seqs", [2, 70])
+def test_row_tiles_in_order_of_length(cuda, seqs, hint):
+    """More row tiles than fit the chip, of chunks that differ in length and prefix: they go out by length, and every one
+    goes out (70 chunks: more than a wave has lanes)."""
+    rng = np.random.default_rng(seqs)
+    chunks = [300, 2100] if seqs == 2 else [int(x) for x in rng.integers(0, 40, seqs - 3)] + [150, 400, 33]
+    prefixes = [2000, 0] if seqs == 2 else [int(x) for x in rng.integers(0, 90, seqs - 3)] + [2100, 30, 0]
+    b = Batch(35, hq=16, hkv=16, dim=64, chunks=chunks, prefixes=prefixes, layers=1, layer=0)
+    q = b.new_rows(b.hq)
+    assert_within(prefill(b, cuda, q, hint=hint), *b.expect_chunks(q))
+
+
 @pytest.mark.parametrize("hq,hkv", [(4, 4), (8, 1)])
 def test_whole_prompts(cuda, hq, hkv):
     b = Batch(32, hq=hq, hkv=hkv, chunks=[300, 1, 257, 512])
