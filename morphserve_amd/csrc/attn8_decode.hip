@@ -180,27 +180,46 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
         after_v();
     };
 
-    int tile = tile_begin + wave;
-    int pid_k = id_of(4 * tile + (n >> 2)), pid_v = id_of(4 * tile + c);
+    // The wave's tiles are tile_begin + wave + 4 k.  Their block ids are read for sixteen tiles at a time, a lane each (lane
+    // 4 k + b: block b of tile k), one such set ahead, and handed out by lane exchange: loads complete in order, and an
+    // id read between a tile's K and V would make the next K wait for this V.
+    const int first = tile_begin + wave;
+    const int count = first < tile_end ? (tile_end - first + 3) >> 2 : 0;
+    auto ids_of = [&](int k0) { return id_of(4 * (first + 4 * (k0 + (lane >> 2))) + (lane & 3)); };
+    int ids = ids_of(0), ids_next = ids_of(16);
+    int pid = -1, pid_k = -1;
     unsigned ex = 0;
-    load_k(x, pid_k);                      // a wave without a tile reads block 0 and uses nothing of it
-    load_v(x, pid_v);
-    ex = scales[max(pid_v, 0)];
-    for (; tile < tile_end; tile += 4) {
-        const int next = min(tile + 4, tile_end);          // behind the last tile: read again, unused
-        const int pid_now = pid_v;
-        const unsigned ex_now = pid_now >= 0 ? ex : 0x7f7fu;
-        pid_k = id_of(4 * next + (n >> 2));
-        pid_v = id_of(4 * next + c);
-        auto after_k = [&] { load_k(x, pid_k); };
-        auto after_v = [&] {
-            load_v(x, pid_v);
-            ex = scales[max(pid_v, 0)];
-        };
-        const bool whole = __ballot(pid_now < 0) == 0 && (tile + 1) * 64 <= len;          // the same for the wave
-        if (whole) consume(std::true_type{}, tile, true, ex_now, after_k, after_v);
-        else consume(std::false_type{}, tile, pid_now >= 0, ex_now, after_k, after_v);
+    auto request_k = [&](int k) {
+        pid_k = __shfl(ids, 4 * (k & 15) + (n >> 2));
+        pid = __shfl(ids, 4 * (k & 15) + c);
+        load_k(x, pid_k);
+        ex = scales[max(pid, 0)];
+    };
+    if (count > 0) {
+        request_k(0);
+        load_v(x, pid);
     }
+    int k = 0;
+    auto step = [&](auto whole_tag) {
+        const bool more = k + 1 < count;
+        const bool here = pid >= 0;
+        auto after_k = [&] {
+            if (!more) return;
+            if (((k + 1) & 15) == 0) {
+                ids = ids_next;
+                ids_next = ids_of(k + 17);
+            }
+            request_k(k + 1);
+        };
+        auto after_v = [&] {
+            if (more) load_v(x, pid);
+        };
+        consume(whole_tag, first + 4 * k, here, here ? ex : 0x7f7fu, after_k, after_v);
+    };
+    // Whole tiles, then, from the first that is not, the careful body: usually the sequence's last tile alone.  Two
+    // loops, not two bodies in one: the accumulators would be copied where the bodies meet.
+    for (; k < count && __ballot(pid < 0) == 0 && (first + 4 * k + 1) * 64 <= len; ++k) step(std::true_type{});
+    for (; k < count; ++k) step(std::false_type{});
 
     // ---- the four waves' states meet in LDS --------------------------------------------------------
     const float l_all = sum_over_quarters(l_run);
