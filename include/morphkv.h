@@ -483,7 +483,7 @@ int mkv_sizeof_batch(void);
  * `position` of cos_table / sin_table ([num_positions, rotary_dim / 2] fp32); head
  * dims >= rotary_dim stay as they are.  k itself is not written.  A row whose
  * position lies outside the tables is not appended and its rotated q is NaN.
- * rotary_dim: a multiple of 16 up to D.  Pointers and strides in multiples of 16
+ * rotary_dim: a multiple of 16 up to D; num_positions at least 1.  Pointers and strides in multiples of 16
  * bytes.  With MKV_ROPE_NONE q, q_out and the tables are ignored. */
 int mkv_store8(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* k,
                const void* v, int64_t k_stride, int64_t v_stride, int32_t layer, int32_t rope,

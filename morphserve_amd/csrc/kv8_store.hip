@@ -5,13 +5,14 @@
 // of one head fit the wave's registers, so the new values are read once and nothing is staged.  Memory bounds a
 // prefill batch (2 bytes in and 1 out an element) and the launch a decode batch.
 //
-//   K, q: a lane holds eight consecutive head dims of a row, 64 such pieces a step; the members of a rotary pair
-//         that lie in another piece are read a second time (from the cache line just fetched) rather than exchanged.
+//   K, q: a lane holds sixteen head dims of a row -- both members of eight rotary pairs, so that a row and its angles are
+//         read once -- and 64 such pieces make a step.
 //   V:    stored transposed, so a lane holds one or two head dims of all sixteen rows and writes their codes as
 //         16 consecutive bytes.
 //
-// The rows a block already held are read again only where a larger scale makes their codes change (K), or where a
-// lane's 16 bytes hold codes that have to survive (V).
+// All of a unit's loads go out before anything waits for one: lanes and steps without a row of their own read one that
+// the unit has, rather than branch.  The rows a block already held are read again only where a larger scale makes their
+// codes change (K), or where a lane's 16 bytes hold codes that have to survive (V).
 #include "kv8.h"
 
 namespace mkv {
@@ -25,10 +26,11 @@ struct Store8Args {
     const float *cos_t, *sin_t;
     int64_t num_positions;
     int32_t layer, num_q_heads, rotary_dim, interleaved;
-    int32_t blocks_per_seq;                                 // grid cells per prefill sequence
+    int32_t blocks_per_seq;                                 // cells per prefill sequence
+    int32_t unit_groups;                                    // workgroups per cell, four units each
 };
 
-// What one grid cell covers: rows [a, b) of block `pid` (its first row is batch row `row`, position 16 j + a).
+// What one cell (decode rows first, then the prefill sequences' blocks) covers: rows [a, b) of block `pid` (its first row is batch row `row`, position 16 j + a).
 struct Cell {
     int64_t pid;          // -1: the rows have no place in the cache
     int64_t row;
@@ -38,14 +40,13 @@ struct Cell {
 };
 
 template <bool ROPE>
-__device__ __forceinline__ bool find_cell(const Store8Args& g, Cell& c) {
+__device__ __forceinline__ bool find_cell(const Store8Args& g, int cell, Cell& c) {
     const mkv_batch& m = g.batch;
-    const int prefill_cells = m.num_prefill_seqs * g.blocks_per_seq;
     int64_t seq_slot;
     int64_t blk;
-    if ((int)blockIdx.x < prefill_cells) {
-        const int s = (int)blockIdx.x / g.blocks_per_seq;
-        const int j = (int)blockIdx.x - s * g.blocks_per_seq;
+    if (cell >= m.num_decoding_seqs) {
+        const int s = (cell - m.num_decoding_seqs) / g.blocks_per_seq;
+        const int j = cell - m.num_decoding_seqs - s * g.blocks_per_seq;
         const int64_t start = m.prefill_start_locs[s];
         const int64_t len = chunk_rows(chunks_of(m), s, start);
         const int64_t prefix = m.prefix_lens ? m.prefix_lens[s] : 0;
@@ -58,7 +59,7 @@ __device__ __forceinline__ bool find_cell(const Store8Args& g, Cell& c) {
         c.row = start + (first - prefix);
         seq_slot = s;
     } else {
-        const int i = (int)blockIdx.x - prefill_cells;
+        const int i = cell;
         const int64_t pos = (int64_t)m.decoding_lens[i] - 1;
         c.row = (int64_t)m.num_prefill_tokens + i;
         blk = pos >= 0 ? pos / kBlk : 0;
@@ -95,78 +96,106 @@ __device__ __forceinline__ float clamped(float x) {
     return __builtin_fabsf(x) > T::kMost ? __builtin_copysignf(T::kMost, x) : x;
 }
 
-// Eight consecutive head dims [8 ch, 8 ch + 8) of a row, rotated by the table row of `pos`.
+// Where the lane's sixteen dims of a row lie: two runs of eight.
+struct Piece {
+    int lo, hi;           // first dims of the runs
+    int table;            // first of the eight table columns; -1: not rotated
+};
+
+template <bool ROPE>
+__device__ __forceinline__ Piece piece_at(const Store8Args& g, int i) {
+    Piece p = {16 * i, 16 * i + 8, -1};
+    if (ROPE && 16 * i < g.rotary_dim) {                             // rotary_dim is a multiple of 16
+        p.table = 8 * i;
+        if (!g.interleaved) {
+            p.lo = 8 * i;
+            p.hi = 8 * i + (g.rotary_dim >> 1);
+        }
+    }
+    return p;
+}
+
+// The piece of one row, rotated by the table row of `pos`: x[0 .. 8) from dim lo, x[8 .. 16) from dim hi.
 template <class T, bool ROPE>
-__device__ __forceinline__ void load_piece(const typename T::elem* row, int ch, int64_t pos, const Store8Args& g,
-                                           float (&x)[8]) {
+__device__ __forceinline__ void load_piece(const typename T::elem* row, const Piece& p, int64_t pos, const Store8Args& g,
+                                           float (&x)[16]) {
     typedef typename T::vec8 vec8;
-    const vec8 own = *(const vec8*)(row + 8 * ch);
+    const vec8 lo = *(const vec8*)(row + p.lo), hi = *(const vec8*)(row + p.hi);
+    float c[8], s[8];
+    if constexpr (ROPE) {
+        const int64_t at = pos * (g.rotary_dim >> 1) + max(p.table, 0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (float)own[e];
+        for (int j = 0; j < 2; ++j) {
+            const float4v cv = *(const float4v*)(g.cos_t + at + 4 * j), sv = *(const float4v*)(g.sin_t + at + 4 * j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                c[4 * j + e] = cv[e];
+                s[4 * j + e] = sv[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = (float)lo[e];
+        x[8 + e] = (float)hi[e];
+    }
     if constexpr (ROPE) {
 #pragma clang fp contract(off)
-        const int R = g.rotary_dim, half = R >> 1;
-        if (8 * ch >= R) return;
-        if (g.interleaved) {
-            const float4v c = *(const float4v*)(g.cos_t + pos * half + 4 * ch);
-            const float4v s = *(const float4v*)(g.sin_t + pos * half + 4 * ch);
+        if (p.table < 0) return;
+        const bool side = g.interleaved;                             // pairs side by side, or eight apart in x
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x0 = x[2 * j], x1 = x[2 * j + 1];
-                const float p0 = x0 * c[j], p1 = x1 * s[j], p2 = x0 * s[j], p3 = x1 * c[j];
-                x[2 * j] = p0 - p1;
-                x[2 * j + 1] = p2 + p3;
-            }
-        } else {
-            const bool upper = 8 * ch >= half;                       // half is a multiple of 8
-            const int d = 8 * ch - (upper ? half : 0);
-            const vec8 other = *(const vec8*)(row + (upper ? d : d + half));
-            float c[8], s[8];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float4v cv = *(const float4v*)(g.cos_t + pos * half + d + 4 * j);
-                const float4v sv = *(const float4v*)(g.sin_t + pos * half + d + 4 * j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    c[4 * j + e] = cv[e];
-                    s[4 * j + e] = sv[e];
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float y = (float)other[e];
-                const float p = x[e] * c[e], r = y * s[e];           // the piece is x0 below half, x1 above
-                x[e] = upper ? r + p : p - r;
+        for (int e = 0; e < 8; ++e) {
+            if (side) {
+                const float x0 = x[2 * e], x1 = x[2 * e + 1];
+                const float p0 = x0 * c[e], p1 = x1 * s[e], p2 = x0 * s[e], p3 = x1 * c[e];
+                x[2 * e] = p0 - p1;
+                x[2 * e + 1] = p2 + p3;
+            } else {
+                const float x0 = x[e], x1 = x[8 + e];
+                const float p0 = x0 * c[e], p1 = x1 * s[e], p2 = x0 * s[e], p3 = x1 * c[e];
+                x[e] = p0 - p1;
+                x[8 + e] = p2 + p3;
             }
         }
     }
 }
 
-template <class T, int D>
+// Rows of the steps.  ONE: the unit has a single row (a decode step's), which the first lanes take in one step.
+template <bool ONE, int PIECES>
+struct Steps {
+    static constexpr int count = ONE ? 1 : kBlk * PIECES / 64;
+    static __device__ __forceinline__ int row(const Cell& c, int lane, int i) { return ONE ? c.a : (lane + 64 * i) / PIECES; }
+    static __device__ __forceinline__ bool mine(int lane) { return !ONE || lane < PIECES; }
+};
+
+template <class T, int D, bool ONE>
 __device__ __forceinline__ void rotate_q(const Store8Args& g, const Cell& c, int head, int lane) {
     typedef typename T::elem E;
-    constexpr int kPieces = D / 8;
+    typedef typename T::vec8 vec8;
+    typedef Steps<ONE, D / 16> S;
+    const Piece p = piece_at<true>(g, lane % (D / 16));
+    float x[S::count][16];
+    // every row is read before any is written: q_out may be q
 #pragma unroll
-    for (int i = 0; i < kBlk * kPieces / 64; ++i) {
-        const int id = lane + 64 * i;
-        const int r = id / kPieces, ch = id % kPieces;
-        // a row's pieces are read by the lanes of one step before any of them is written: q_out may be q
-        if (r < c.a || r >= c.b) continue;
-        const int64_t row = c.row + (r - c.a);
-        const E* src = (const E*)g.q + row * g.q_stride + (int64_t)head * D;
-        float x[8];
-        if (r < c.b_known) {
-            load_piece<T, true>(src, ch, c.pos0 + r, g, x);
-        } else {
-            load_piece<T, false>(src, ch, 0, g, x);
+    for (int i = 0; i < S::count; ++i) {
+        const int r = min(max(S::row(c, lane, i), c.a), c.b - 1);
+        const int64_t pos = r < c.b_known ? c.pos0 + r : 0;
+        load_piece<T, true>((const E*)g.q + (c.row + (r - c.a)) * g.q_stride + (int64_t)head * D, p, pos, g, x[i]);
+    }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (8 * ch < g.rotary_dim) x[e] = __builtin_nanf("");
+    for (int i = 0; i < S::count; ++i) {
+        const int r = S::row(c, lane, i);
+        if (!S::mine(lane) || r < c.a || r >= c.b) continue;
+        const bool lost = r >= c.b_known && p.table >= 0;            // no angle for this row
+        vec8 lo, hi;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            lo[e] = (E)(lost ? __builtin_nanf("") : x[i][e]);
+            hi[e] = (E)(lost ? __builtin_nanf("") : x[i][8 + e]);
         }
-        typename T::vec8 o;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = (E)x[e];
-        *(typename T::vec8*)((E*)g.q_out + row * g.q_out_stride + (int64_t)head * D + 8 * ch) = o;
+        E* dst = (E*)g.q_out + (c.row + (r - c.a)) * g.q_out_stride + (int64_t)head * D;
+        *(vec8*)(dst + p.lo) = lo;
+        *(vec8*)(dst + p.hi) = hi;
     }
 }
 
@@ -177,112 +206,115 @@ __device__ __forceinline__ unsigned joined_exponent(float amax, bool fresh, unsi
     return fresh ? e : max(e, had);
 }
 
-template <class T, class C, int D, bool ROPE>
+// Four codes of an older scale at the new one.
+template <class C>
+__device__ __forceinline__ unsigned moved4(unsigned w, float again) {
+    float y[4];
+    C::decode4(w, y);
+    return C::encode4(y[0] * again, y[1] * again, y[2] * again, y[3] * again);
+}
+
+template <class T, class C, int D, bool ROPE, bool ONE>
 __device__ __forceinline__ void store_k(const Store8Args& g, const Cell& c, int kvh, int lane) {
     typedef typename T::elem E;
-    constexpr int kPieces = D / 8, kSteps = kBlk * kPieces / 64;
-    float x[kSteps][8];
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const int id = lane + 64 * i;
-        const int r = id / kPieces, ch = id % kPieces;
-        if (r >= c.a && r < c.b_known) {
-            const E* src = (const E*)g.k + (c.row + (r - c.a)) * g.k_stride + (int64_t)kvh * D;
-            load_piece<T, ROPE>(src, ch, c.pos0 + r, g, x[i]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[i][e] = clamped<T>(x[i][e]);
-                amax = fmaxf(amax, __builtin_fabsf(x[i][e]));        // a NaN does not enter
-            }
-        }
-    }
-    amax = wave_max(amax);
+    typedef Steps<ONE, D / 16> S;
+    const Piece p = piece_at<ROPE>(g, lane % (D / 16));
     uint8_t* scale = (uint8_t*)(scale_row8(g.pool, g.layer, kvh) + c.pid);
     const unsigned had = scale[0];
+    float x[S::count][16];
+    float amax = 0.f;
+    // a row outside the unit's is read as its nearest one, which the maximum does not mind
+#pragma unroll
+    for (int i = 0; i < S::count; ++i) {
+        const int r = min(max(S::row(c, lane, i), c.a), c.b_known - 1);
+        load_piece<T, ROPE>((const E*)g.k + (c.row + (r - c.a)) * g.k_stride + (int64_t)kvh * D, p, c.pos0 + r, g, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < S::count; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            x[i][e] = clamped<T>(x[i][e]);
+            amax = fmaxf(amax, __builtin_fabsf(x[i][e]));            // a NaN does not enter
+        }
+    amax = wave_max(amax);
     const unsigned e8 = joined_exponent<C>(amax, c.a == 0, had);
     const float inv = pow2_of(254u - min(e8, 253u));
-    const float again = pow2_of(had) * inv;                          // older codes to the new scale
     uint8_t* slab = (uint8_t*)g.pool.k + c.pid * block_bytes8(g.pool) + slab_offset8(g.pool, g.layer, kvh);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const int id = lane + 64 * i;
-        const int r = id / kPieces, ch = id % kPieces;
-        uint2* at = (uint2*)(slab + r * D + 8 * ch);
-        if (r >= c.a && r < c.b_known) {
-            float y[8];
+    for (int i = 0; i < S::count; ++i) {
+        const int r = S::row(c, lane, i);
+        if (!S::mine(lane) || r < c.a || r >= c.b_known) continue;
+        float y[16];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[i][e] * inv;
-            *at = make_uint2(C::encode4(y[0], y[1], y[2], y[3]), C::encode4(y[4], y[5], y[6], y[7]));
-        } else if (r < c.a && e8 != had) {
-            const uint2 old = *at;
-            float y[4], z[4];
-            C::decode4(old.x, y);
-            C::decode4(old.y, z);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y[e] *= again;
-                z[e] *= again;
-            }
-            *at = make_uint2(C::encode4(y[0], y[1], y[2], y[3]), C::encode4(z[0], z[1], z[2], z[3]));
+        for (int e = 0; e < 16; ++e) y[e] = x[i][e] * inv;
+        *(uint2*)(slab + r * D + p.lo) = make_uint2(C::encode4(y[0], y[1], y[2], y[3]), C::encode4(y[4], y[5], y[6], y[7]));
+        *(uint2*)(slab + r * D + p.hi) = make_uint2(C::encode4(y[8], y[9], y[10], y[11]), C::encode4(y[12], y[13], y[14], y[15]));
+    }
+    if (c.a > 0 && e8 != had) {                                      // the same for the wave
+        const float again = pow2_of(had) * inv;                      // older codes to the new scale
+        for (int u = lane; u < c.a * (D / 16); u += 64) {
+            uint4* at = (uint4*)slab + u;
+            const uint4 w = *at;
+            *at = make_uint4(moved4<C>(w.x, again), moved4<C>(w.y, again), moved4<C>(w.z, again), moved4<C>(w.w, again));
         }
     }
     if (lane == 0) scale[0] = (uint8_t)e8;
 }
 
-template <class T, class C, int D>
+template <class T, class C, int D, bool ONE>
 __device__ __forceinline__ void store_v(const Store8Args& g, const Cell& c, int kvh, int lane) {
     typedef typename T::elem E;
     constexpr int kDims = D / 64;                                    // head dims per lane
+    constexpr int kN = ONE ? 1 : kBlk;                               // rows read
     typedef E vecd __attribute__((ext_vector_type(kDims)));
-    float x[kDims][kBlk];
-    float amax = 0.f;
     const E* src = (const E*)g.v + (int64_t)kvh * D + lane * kDims;
-#pragma unroll
-    for (int r = 0; r < kBlk; ++r) {
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) x[d][r] = 0.f;
-        if (r >= c.a && r < c.b_known) {                             // the same for the whole wave
-            const vecd y = *(const vecd*)(src + (c.row + (r - c.a)) * g.v_stride);
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) {
-                x[d][r] = clamped<T>((float)y[d]);
-                amax = fmaxf(amax, __builtin_fabsf(x[d][r]));
-            }
-        }
-    }
-    amax = wave_max(amax);
     uint8_t* scale = (uint8_t*)(scale_row8(g.pool, g.layer, kvh) + c.pid) + 1;
     const unsigned had = *scale;
+    uint4* at = (uint4*)((uint8_t*)g.pool.v + c.pid * block_bytes8(g.pool) + slab_offset8(g.pool, g.layer, kvh)) + lane * kDims;
+    const bool whole = !ONE && c.a == 0 && c.b_known == kBlk;
+    vecd y[kN];
+#pragma unroll
+    for (int r = 0; r < kN; ++r) {
+        const int rr = ONE ? c.a : min(max(r, c.a), c.b_known - 1);
+        y[r] = *(const vecd*)(src + (c.row + (rr - c.a)) * g.v_stride);
+    }
+    uint4 held[kDims];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) held[d] = whole ? make_uint4(0u, 0u, 0u, 0u) : at[d];
+    float x[kDims][kN];
+    float amax = 0.f;
+#pragma unroll
+    for (int r = 0; r < kN; ++r)
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+            x[d][r] = clamped<T>((float)y[r][d]);
+            amax = fmaxf(amax, __builtin_fabsf(x[d][r]));
+        }
+    amax = wave_max(amax);
     const unsigned e8 = joined_exponent<C>(amax, c.a == 0, had);
     const float inv = pow2_of(254u - min(e8, 253u));
     const float again = pow2_of(had) * inv;
-    uint4v* at = (uint4v*)((uint8_t*)g.pool.v + c.pid * block_bytes8(g.pool) + slab_offset8(g.pool, g.layer, kvh)) + lane * kDims;
-    const bool whole = c.a == 0 && c.b_known == kBlk;
+    const bool moves = c.a > 0 && e8 != had;
+    // of each word's four rows: those below a take their moved codes, [a, b) the new ones, those behind stay
+    auto word = [&](unsigned w, unsigned fresh, int n) {
+        auto below = [n](int r) {
+            const int in = min(max(r - 4 * n, 0), 4);
+            return in >= 4 ? ~0u : (1u << (8 * in)) - 1u;
+        };
+        const unsigned old = below(c.a), upto = below(c.b_known);
+        if (moves) w = (w & ~old) | (moved4<C>(w, again) & old);
+        return (w & ~(upto & ~old)) | (fresh & upto & ~old);
+    };
 #pragma unroll
     for (int d = 0; d < kDims; ++d) {
-        uint4v w = {0u, 0u, 0u, 0u};
-        if (!whole) w = at[d];
+        unsigned fresh[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const unsigned fresh = C::encode4(x[d][4 * n] * inv, x[d][4 * n + 1] * inv, x[d][4 * n + 2] * inv, x[d][4 * n + 3] * inv);
-            unsigned kept = w[n];
-            if (!whole && 4 * n < c.a && e8 != had) {
-                float y[4];
-                C::decode4(kept, y);
-                const unsigned moved = C::encode4(y[0] * again, y[1] * again, y[2] * again, y[3] * again);
-                // rows below a take their moved codes; what lies behind the cell's rows stays
-                const int below = min(c.a - 4 * n, 4);
-                const unsigned mask = below >= 4 ? ~0u : (1u << (8 * below)) - 1u;
-                kept = (kept & ~mask) | (moved & mask);
-            }
-            const int lo = min(max(c.a - 4 * n, 0), 4), hi = min(max(c.b_known - 4 * n, 0), 4);
-            const unsigned to_hi = hi >= 4 ? ~0u : (1u << (8 * hi)) - 1u;
-            const unsigned to_lo = lo >= 4 ? ~0u : (1u << (8 * lo)) - 1u;
-            const unsigned mask = to_hi & ~to_lo;
-            w[n] = (kept & ~mask) | (fresh & mask);
+            if (ONE) fresh[n] = n ? fresh[0] : C::encode4(x[d][0] * inv, x[d][0] * inv, x[d][0] * inv, x[d][0] * inv);
+            else fresh[n] = C::encode4(x[d][(4 * n) % kN] * inv, x[d][(4 * n + 1) % kN] * inv, x[d][(4 * n + 2) % kN] * inv, x[d][(4 * n + 3) % kN] * inv);
         }
-        at[d] = w;
+        if (whole) at[d] = make_uint4(fresh[0], fresh[1], fresh[2], fresh[3]);
+        else at[d] = make_uint4(word(held[d].x, fresh[0], 0), word(held[d].y, fresh[1], 1), word(held[d].z, fresh[2], 2), word(held[d].w, fresh[3], 3));
     }
     if (lane == 0) *scale = (uint8_t)e8;
 }
@@ -290,17 +322,22 @@ __device__ __forceinline__ void store_v(const Store8Args& g, const Cell& c, int 
 template <class T, class C, int D, bool ROPE>
 __global__ __launch_bounds__(256) void store8_kernel(const Store8Args g) {
     const int lane = threadIdx.x & 63;
-    // unit: K heads, V heads, then q heads
-    int unit = __builtin_amdgcn_readfirstlane((int)blockIdx.y * 4 + (int)(threadIdx.x >> 6));
+    // unit: K heads, V heads, then q heads.  The heads of a cell are consecutive workgroups: together they read whole rows.
+    const int cell = (int)(blockIdx.x / (unsigned)g.unit_groups);
+    const int unit = __builtin_amdgcn_readfirstlane(((int)blockIdx.x - cell * g.unit_groups) * 4 + (int)(threadIdx.x >> 6));
     const int Hkv = g.pool.num_kv_heads;
     Cell c;
-    if (!find_cell<ROPE>(g, c)) return;
+    if (!find_cell<ROPE>(g, cell, c)) return;
     if (unit < 2 * Hkv) {
         if (c.pid < 0 || c.b_known <= c.a) return;
-        if (unit < Hkv) store_k<T, C, D, ROPE>(g, c, unit, lane);
-        else store_v<T, C, D>(g, c, unit - Hkv, lane);
+        const bool one = c.b_known - c.a == 1;
+        if (unit < Hkv && one) store_k<T, C, D, ROPE, true>(g, c, unit, lane);
+        else if (unit < Hkv) store_k<T, C, D, ROPE, false>(g, c, unit, lane);
+        else if (one) store_v<T, C, D, true>(g, c, unit - Hkv, lane);
+        else store_v<T, C, D, false>(g, c, unit - Hkv, lane);
     } else if (ROPE && unit < 2 * Hkv + g.num_q_heads) {
-        rotate_q<T, D>(g, c, unit - 2 * Hkv, lane);
+        if (c.b - c.a == 1) rotate_q<T, D, true>(g, c, unit - 2 * Hkv, lane);
+        else rotate_q<T, D, false>(g, c, unit - 2 * Hkv, lane);
     }
 }
 
@@ -378,7 +415,7 @@ int mkv_store8(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, con
         MKV_REQUIRE(num_q_heads > 0 && num_q_heads <= 65535, "num_q_heads %d outside the supported range", num_q_heads);
         MKV_REQUIRE(rotary_dim > 0 && rotary_dim <= pool->head_dim && rotary_dim % 16 == 0,
                     "rotary_dim %d must be a multiple of 16 within head_dim %d", rotary_dim, pool->head_dim);
-        MKV_REQUIRE(num_positions >= 0, "num_positions must be >= 0");
+        MKV_REQUIRE(num_positions > 0, "the rotary tables hold no position");
         MKV_REQUIRE((((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)cos_table | (uintptr_t)sin_table) & 15) == 0 &&
                         ((q_stride | q_out_stride) & 7) == 0,
                     "q rows and the rotary tables must be 16-byte aligned");
@@ -398,8 +435,9 @@ int mkv_store8(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, con
     // a chunk behind a prefix may begin inside a block: one cell more
     g.blocks_per_seq = prefill ? mkv::cdiv(batch->max_prefill_len, mkv::kBlk) + (batch->prefix_lens ? 1 : 0) : 0;
     const int64_t cells = (int64_t)batch->num_prefill_seqs * g.blocks_per_seq + batch->num_decoding_seqs;
-    MKV_REQUIRE(cells <= 0x7fffffff, "too many rows in one call");
-    const dim3 grid((unsigned)cells, (unsigned)mkv::cdiv(units, 4));
+    g.unit_groups = mkv::cdiv(units, 4);
+    MKV_REQUIRE(cells * g.unit_groups <= 0x7fffffff, "too many rows in one call");
+    const dim3 grid((unsigned)(cells * g.unit_groups));
     hipStream_t s = (hipStream_t)stream;
     const bool rot = rope != MKV_ROPE_NONE;
     if (dtype == MKV_F16) {

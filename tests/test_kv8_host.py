@@ -190,7 +190,7 @@ def test_bad_pools_and_batches(entry):
 @pytest.mark.parametrize("bad", [dict(k=None), dict(v=None), dict(k=A + 8), dict(vs=516), dict(rope=3), dict(b=batch8(decoding_lens=None)),
                                  dict(b=batch8(prefill_lens=None)), dict(rope=1, q=None), dict(rope=1, cos=None), dict(rope=1, rotary=24),
                                  dict(rope=2, rotary=0), dict(rope=1, rotary=144), dict(rope=1, hq=0), dict(rope=1, q=A + 2),
-                                 dict(rope=1, qs=513), dict(rope=1, sin=A + 4), dict(rope=1, positions=-1), dict(rope=1, qos=1024)])
+                                 dict(rope=1, qs=513), dict(rope=1, sin=A + 4), dict(rope=1, positions=-1), dict(rope=1, positions=0), dict(rope=1, qos=1024)])
 def test_bad_store(bad):
     assert store(**bad) == _capi.MKV_EINVAL
     assert _capi.lib().mkv_last_error()
