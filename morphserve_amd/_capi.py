@@ -230,6 +230,35 @@ def use_diag_library():
         _lib = saved
 
 
+_binding = None
+_entries: dict = {}
+
+
+def binding():
+    """The native host side of the 8-bit and rotary operators (``csrc/binding.cpp``), loaded once."""
+    global _binding
+    if _binding is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (its libraries are the module's)
+        path = os.path.join(_HERE, "csrc", "_binding.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it with `python -m morphserve_amd.csrc.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_binding", path)
+        _binding = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+        loader.exec_module(_binding)
+    return _binding
+
+
+def entry(name: str) -> int:
+    """Address of an entry point of the library that calls go through at the moment."""
+    key = (name, lib())
+    address = _entries.get(key)
+    if address is None:
+        address = _entries[key] = C.cast(getattr(key[1], name), C.c_void_p).value
+    return address
+
+
 def check(rc: int) -> None:
     if rc != MKV_OK:
         raise MorphKVError(rc, lib().mkv_last_error().decode("utf-8", "replace"))

@@ -6,6 +6,9 @@ plus ``diag.hip``: the same entry points and, on top, the switches and measureme
 ``include/morphkv_diag.h`` (kernel variants, per-launch event timing, per-workgroup time stamps,
 calibration loops).  Benchmarks and tests that need those load the twin; the package never does.
 
+``_binding.so`` is the host side of the 8-bit cache's and the rotary operators (argument checks and the call, a CPython
+module over torch's C++ tensors); it holds no kernel and takes the library's entries by address.
+
 Usage: ``python -m morphserve_amd.csrc.build`` or ``build_library()``.
 The shared objects land next to the sources so that they travel with the tree.
 """
@@ -23,6 +26,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "libmorphkv.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 DIAG_LIB_PATH = os.path.join(HERE, "libmorphkv_diag.so")
+BINDING_PATH = os.path.join(HERE, "_binding.so")
 
 SOURCES = [
     "core.hip",
@@ -69,6 +73,24 @@ def _compile(src: str, obj_dir: str, defines=()) -> str:
     return obj
 
 
+def _build_binding() -> None:
+    import sysconfig
+    from torch.utils.cpp_extension import include_paths
+    import torch
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = BINDING_PATH + ".tmp"
+    cmd = [_hipcc(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-x", "c++",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I" + INCLUDE,
+           "-I" + os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_hipcc()))), "include"),
+           *("-I" + p for p in include_paths()), "-I" + sysconfig.get_paths()["include"],
+           os.path.join(HERE, "binding.cpp"), "-o", tmp, "-L" + libs, "-ltorch_python", "-ltorch_cpu", "-ltorch_hip",
+           "-lc10", "-lc10_hip"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"hipcc failed for binding.cpp:\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+
+
 def _link(objs, out: str) -> None:
     tmp = out + ".tmp"
     cmd = [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC",
@@ -80,8 +102,8 @@ def _link(objs, out: str) -> None:
 
 
 def build_library(verbose: bool = True, jobs: int = 8, diag: bool = True) -> str:
-    """Compile every source and link ``libmorphkv.so`` (and, with ``diag``, its diagnostic twin);
-    always rebuilds."""
+    """Compile every source and link ``libmorphkv.so`` (and, with ``diag``, its diagnostic twin)
+    and ``_binding.so``; always rebuilds."""
     obj_dir = os.path.join(HERE, "build")
     diag_dir = os.path.join(obj_dir, "diag")
     os.makedirs(diag_dir if diag else obj_dir, exist_ok=True)
@@ -91,12 +113,14 @@ def build_library(verbose: bool = True, jobs: int = 8, diag: bool = True) -> str
     # the attention files dominate the build: start them first
     work.sort(key=lambda w: 0 if "attn" in w[0] else 1)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        binding = ex.submit(_build_binding)
         objs = list(ex.map(lambda w: (w[1], _compile(*w)), work))
+        binding.result()
     _link([o for d, o in objs if d == obj_dir], LIB_PATH)
     if diag:
         _link([o for d, o in objs if d == diag_dir], DIAG_LIB_PATH)
     if verbose:
-        for path in (LIB_PATH, DIAG_LIB_PATH) if diag else (LIB_PATH,):
+        for path in (LIB_PATH, DIAG_LIB_PATH, BINDING_PATH) if diag else (LIB_PATH, BINDING_PATH):
             print(f"built {path} ({os.path.getsize(path) / 1024:.0f} KiB)")
     return LIB_PATH
 

@@ -18,7 +18,7 @@ import torch
 
 from . import _capi
 
-KINDS = {torch.float8_e4m3fn: _capi.KV8_E4M3, torch.int8: _capi.KV8_INT8}
+KINDS = (torch.float8_e4m3fn, torch.int8)
 
 
 @dataclasses.dataclass
@@ -29,36 +29,13 @@ class KV8Cache:
     v: torch.Tensor
     scales: torch.Tensor
 
-    def __post_init__(self):
-        self._pool = None
-
     @property
     def num_blocks(self) -> int:
         return self.k.shape[0]
 
     def descriptor(self) -> _capi.MkvPool8:
-        """The cache as the C entries take it.  The tensors are checked the first time and must not be exchanged
-        afterwards: make another ``KV8Cache`` for other tensors."""
-        if self._pool is None:
-            k, v, scales = self.k, self.v, self.scales
-            dtype, shape, device = k.dtype, k.shape, k.device
-            if dtype not in KINDS or v.dtype != dtype:
-                raise ValueError(f"an 8-bit cache holds float8_e4m3fn or int8 codes, got {dtype} / {v.dtype}")
-            if len(shape) != 5 or 0 in shape:
-                raise ValueError(f"k must be [num_blocks, L, Hkv, block_size, D], got {tuple(shape)}")
-            n, layers, heads, block, dim = shape
-            if v.shape != (n, layers, heads, dim, block):
-                raise ValueError(f"v must be {(n, layers, heads, dim, block)}, got {tuple(v.shape)}")
-            if scales.dtype != torch.uint8 or scales.shape != (layers, heads, n, 2):
-                raise ValueError(f"scales must be uint8 {(layers, heads, n, 2)}, got {scales.dtype} {tuple(scales.shape)}")
-            if not (k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
-                raise ValueError("the tensors of an 8-bit cache must be contiguous")
-            if v.device != device or scales.device != device:
-                raise ValueError("the tensors of an 8-bit cache must be on one device")
-            self.shape, self.device = tuple(shape), device
-            self._pool = _capi.MkvPool8(k.data_ptr(), v.data_ptr(), scales.data_ptr(), n, layers, heads, block, dim,
-                                        KINDS[dtype], 0)
-        return self._pool
+        """The cache as the C entries of include/morphkv.h take it; ``ValueError`` if the tensors do not make one."""
+        return _capi.MkvPool8(*_capi.binding().pool_fields(self.k, self.v, self.scales))
 
 
 def allocate_kv8_cache(num_blocks: int, shape_tail: Sequence[int], dtype: torch.dtype = torch.float8_e4m3fn,

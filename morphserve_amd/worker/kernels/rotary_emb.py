@@ -151,27 +151,4 @@ def rotary_embedding(
 ) -> None:
     """Rotates the first ``rotary_dim`` dims of every head by its token's position, in 32 bits, and keeps the others.  A
     token whose position lies outside the tables gets NaN in its rotated dims."""
-    from .kv8 import DTYPES, _ints, _layout, _on, _out_rows, _rows, _stream, _tables
-    dtype, dev = q.dtype, q.device
-    if q.dim() != 3 or dtype not in DTYPES or dev.type != "cuda":
-        raise ValueError(f"q must be [tokens, heads, dim] float16 or bfloat16 on the GPU, got {dtype} {tuple(q.shape)} on {dev}")
-    rope = _layout(layout)
-    tokens, heads, dim = q.shape
-    q_out = q if q_out is None else q_out
-    qs, qos = _rows(q, "q", dtype, dev, tokens, heads, dim), _out_rows(q_out, "q_out", dtype, dev, tokens, heads, dim)
-    kv_heads, ks, kos, k_ptr, k_out_ptr = 0, 0, 0, None, None
-    if k is not None:
-        if k.dim() != 3:
-            raise ValueError(f"k must be [tokens, heads, dim], got {tuple(k.shape)}")
-        k_out = k if k_out is None else k_out
-        kv_heads = k.shape[1]
-        ks, kos = _rows(k, "k", dtype, dev, tokens, kv_heads, dim), _out_rows(k_out, "k_out", dtype, dev, tokens, kv_heads, dim)
-        k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
-    if positions.shape != (tokens,):
-        raise ValueError(f"positions must be [{tokens}], got {tuple(positions.shape)}")
-    pos = _ints(positions, "positions", dev, tokens)
-    rows, rotary_dim = _tables(cos, sin, dev)
-    with _on(dev):
-        _capi.check(_capi.lib().mkv_rope_positions(
-            DTYPES[dtype], rope, q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, qs, ks, qos, kos, pos, cos.data_ptr(),
-            sin.data_ptr(), rows, tokens, heads, kv_heads, dim, rotary_dim, _stream(dev)))
+    _capi.check(_capi.binding().rope(_capi.entry("mkv_rope_positions"), q, k, positions, cos, sin, layout, q_out, k_out))

@@ -179,7 +179,7 @@ def test_decode_groups(cuda, group):
 def test_decode_splits(cuda, monkeypatch, dtype, kind, splits):
     """The same lengths cut into few and many ranges, empty ones and a bound that is too small among them."""
     b = Batch(12, hq=6, hkv=2, dtype=dtype, kind=kind, dec=[1, 64, 130, 0, 700, 2600, 65])
-    monkeypatch.setattr(kv8, "choose_split_8bit", lambda *a, **k: (64, splits))
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
     q = b.new_rows(b.hq)
     assert_within(decode(b, cuda, q), *b.expect_decode(q))
 
@@ -282,7 +282,7 @@ def test_chunks(cuda, dtype, kind, dim, hq, hkv):
 @pytest.mark.parametrize("dtype,kind", TYPES)
 def test_chunks_split_over_the_keys(cuda, monkeypatch, dtype, kind, splits):
     b = Batch(31, hq=6, hkv=2, dtype=dtype, kind=kind, **CHUNKS)
-    monkeypatch.setattr(kv8, "choose_prefill_split_8bit", lambda *a, **k: (64, splits))
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
     q = b.new_rows(b.hq)
     assert_within(prefill(b, cuda, q), *b.expect_chunks(q))
 
@@ -324,7 +324,7 @@ def test_chunks_with_missing_blocks(cuda):
 @pytest.mark.parametrize("splits", [1, 3])
 def test_rows_of_no_chunk_stay(cuda, monkeypatch, splits):
     """Rows between and behind the chunks are neither read nor written."""
-    monkeypatch.setattr(kv8, "choose_prefill_split_8bit", lambda *a, **k: (64, splits))
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
     b = Batch(34, hq=4, hkv=2, chunks=[20, 33], prefixes=[10, 100])
     q = b.new_rows(b.hq)
     want, bound = b.expect_chunks(q)

@@ -119,7 +119,7 @@ def test_cache_object():
     cache = allocate_kv8_cache(5, (2, 3, 16, 64), torch.int8, "cpu")
     pool = cache.descriptor()
     assert (pool.num_blocks, pool.num_layers, pool.num_kv_heads, pool.block_size, pool.head_dim, pool.kind) == (5, 2, 3, 16, 64, 1)
-    assert pool is cache.descriptor() and pool.k == cache.k.data_ptr() and cache.num_blocks == 5
+    assert (pool.k, pool.v, pool.scales) == tuple(t.data_ptr() for t in (cache.k, cache.v, cache.scales)) and cache.num_blocks == 5
     k, v, s = cache.k, cache.v, cache.scales
     for bad in ((k.half(), v.half(), s), (k, v.view(torch.uint8), s), (k, k, s), (k, v, s[:1]), (k, v, s.int()),
                 (k[:, :, :, :, :32], v[:, :, :, :32], s), (k[:0], v[:0], s[:, :, :0]), (k[0], v[0], s), (k[::2], v[::2], s[:, :, ::2])):
