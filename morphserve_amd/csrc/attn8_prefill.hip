@@ -1,8 +1,8 @@
 // Chunked prefill attention over the 8-bit paged cache.
 //
-// The rows of one kv head -- chunk positions times the q heads that share it, position-major -- are cut into tiles
-// of 64 to 256, one workgroup of four or eight waves each; a wave owns one or two 16-row column tiles.  Keys come 64 at a time (four
-// blocks): their codes are converted once, on the way into LDS, and every wave reads the converted tile from there,
+// The rows of one kv head -- chunk positions times the q heads that share it, position-major -- are cut into tiles of 64
+// to 256, one workgroup of four or eight waves each; a wave owns one or two 16-row column tiles.  Keys come 64 at a time
+// (four blocks): their codes are converted once, on the way into LDS, and every wave reads the converted tile from there,
 //
 //   S^T[key, row] = K . Q^T        v_mfma_f32_16x16x32
 //   O^T[dim, row] += V^T . P^T     v_mfma_f32_16x16x32
@@ -11,6 +11,11 @@
 // decode kernel the keys are numbered so that lane group c scores block c in order, which makes K's scale one factor
 // per lane and the scores, exponentiated, the operand of the second product.  V arrives transposed from the cache,
 // so that both products read LDS in rows.  Where few rows meet many keys, the keys are cut into splits.
+//
+// Bound: the matrix cores where rows are many -- 2048 tokens of 32 q heads after 8192 cached ones take 370 us, 835 TFLOP/s
+// of the two products, whole prompts of 8192 tokens 623 us (882) -- less what the softmax leaves them idle: the two waves of
+// a SIMD alternate between products and exponentials.  A wave reads its operands from LDS four ahead of the products, K's
+// last ones already V's first, and nothing is loaded under a condition, since waits where two paths meet take the worse one.
 #include <type_traits>
 
 #include "kv8.h"
@@ -20,12 +25,9 @@ namespace mkv {
 static constexpr int kVAhead = 4;             // V operands requested ahead of the softmax
 static constexpr float kLazyP = 8.f;
 
-// three-input maximum in one instruction (two of the two-input kind each canonicalise their operands first)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
+// The larger of two numbers as the median of them and infinity: one instruction, where fmaxf first makes its operands
+// canonical -- and one that the compiler knows to read a matrix product's result.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
 
 struct Prefill8Args {
     mkv_pool8 pool;
@@ -127,47 +129,26 @@ __device__ __forceinline__ bool nth_longest(const Prefill8Args& g, int per, int 
     return false;
 }
 
+// A workgroup's row tile against its range of the keys: rows row0 .. of the `rows` of chunk b, starting at batch row `start`.
 template <class T, class C, int D, int WAVES, int COLS>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn8_prefill_kernel(const Prefill8Args g) {
+__device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)[Lds8<D>::kK], char (*v_lds)[Lds8<D>::kV], int b,
+                                            int split, int kvh, int64_t start, int rows, int row0) {
     typedef typename T::elem E;
     typedef typename T::vec8 vec8;
     typedef E vec4 __attribute__((ext_vector_type(4)));
     typedef Lds8<D> L;
     constexpr int kThreads = 64 * WAVES;
-    constexpr int kRows = 16 * COLS * WAVES;                 // rows per workgroup
+    constexpr int kRows = 16 * COLS * WAVES;                  // rows of the tile
     constexpr int kX = D / 32, kT = D / 16;                   // steps of the first product, dim tiles of the second
     constexpr int kUnits = 4 * D;                             // 16-byte units of a tile's K (and V) slabs
     constexpr int kU = kUnits >= kThreads ? kUnits / kThreads : 1;
-    __shared__ __attribute__((aligned(16))) char k_lds[2][L::kK];
-    __shared__ __attribute__((aligned(16))) char v_lds[2][L::kV];
-
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15;
     const int c = lane >> 4;
-    // Workgroups are numbered (row tile, split, kv head), the head fastest: consecutive ones go to the eight XCDs in
-    // turn, so that with eight kv heads or a multiple a head's row tiles share one L2.
-    const int Hkv = g.pool.num_kv_heads;
     const int G = g.group;
-    const int Hq = Hkv * G;
-    const int cell = (int)(blockIdx.x / (unsigned)Hkv);
-    const int kvh = (int)blockIdx.x - cell * Hkv;
-    const int job = cell / g.max_splits;
-    const int split = cell - job * g.max_splits;
-    int b, rank;                                              // rank: the row tile, counted from the chunk's last
-    if (g.sorted) {
-        if (!nth_longest(g, kRows, job, lane, b, rank)) return;
-    } else {
-        rank = job / g.batch.num_prefill_seqs;
-        b = job - rank * g.batch.num_prefill_seqs;
-    }
-    const int64_t start = g.batch.prefill_start_locs[b];
-    const int len = chunk_rows(chunks_of(g.batch), b, start);
-    const int rows = len * G;
-    const int tiles = (rows + kRows - 1) / kRows;             // of this chunk
-    if (rank >= tiles) return;
-    const int row0 = (tiles - 1 - rank) * kRows;
+    const int Hq = g.pool.num_kv_heads * G;
     const int64_t seq = g.batch.seq_ids[b];
     const bool has_row = seq >= 0 && seq < g.batch.table_rows;
     const int64_t prefix = g.batch.prefix_lens ? max(g.batch.prefix_lens[b], 0) : 0;
@@ -219,55 +200,57 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const uint16_t* scales = scale_row8(g.pool, g.layer, kvh);
 
     // ---- staging: unit w of a tile's slabs belongs to block w / D; a thread takes units tid, tid + kThreads, ... ---------
-    auto id_of = [&](int blk) {
-        const int pid = blk < nblk ? table[blk] : -1;
-        return pid >= 0 && pid < num_blocks ? pid : -1;
-    };
-    const bool stages = tid < kUnits;                         // the same for a wave
+    auto unit = [&](int u) { return (tid + kThreads * u) % kUnits; };       // more threads than units: some twice
+    // Ids are kept as the table holds them and looked at when they are used, a tile later: loads complete in order, and a
+    // glance at an id that was just asked for would wait for the codes asked for before it.
+    auto ask_id = [&](int blk) { return table[min(blk, nblk - 1)]; };
+    auto known_id = [&](int blk, int id) { return blk < nblk && id >= 0 && id < num_blocks ? id : -1; };
     uint4v kreg[kU], vreg[kU];
     int valid[kU];                                            // keys of the units' blocks that count
     unsigned ereg[kU];                                        // the blocks' exponents
     int ids[kU], id_c;                                        // of the tile after the fetched one: units' blocks, block c
     bool here = false, here_next = false;                     // block c of the current / fetched tile
     unsigned ex = 0, ex_next = 0;
-    auto load_ids = [&](int tile) {
+    auto ask_ids = [&](int tile) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) ids[u] = id_of(4 * tile + (tid + kThreads * u) / D);
-        id_c = id_of(4 * tile + c);
+        for (int u = 0; u < kU; ++u) ids[u] = ask_id(4 * tile + unit(u) / D);
+        id_c = ask_id(4 * tile + c);
     };
     // requests the codes of `tile` and the ids of the one after it
     auto fetch = [&](int tile) {
-        if (stages) {
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int64_t at = (int64_t)max(ids[u], 0) * block_bytes + 16 * ((tid + kThreads * u) % D);
-                kreg[u] = *(const uint4v*)(k_base + at);
-                vreg[u] = *(const uint4v*)(v_base + at);
-                ereg[u] = scales[max(ids[u], 0)];
-                valid[u] = ids[u] >= 0 ? min(max(kv_len - (4 * tile + (tid + kThreads * u) / D) * kBlk, 0), kBlk) : 0;
-            }
-        }
-        ex_next = scales[max(id_c, 0)];
-        here_next = id_c >= 0;
-        load_ids(tile + 1);                                   // past the end: no block
-    };
-    auto stage = [&](int buf) {
-        if (!stages) return;
+        const int own = known_id(4 * tile + c, id_c);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int w = tid + kThreads * u;
+            const int blk = 4 * tile + unit(u) / D;
+            const int id = known_id(blk, ids[u]);
+            const int64_t at = (int64_t)max(id, 0) * block_bytes + 16 * (unit(u) % D);
+            kreg[u] = *(const uint4v*)(k_base + at);
+            vreg[u] = *(const uint4v*)(v_base + at);
+            ereg[u] = scales[max(id, 0)];
+            valid[u] = id >= 0 ? min(max(kv_len - blk * kBlk, 0), kBlk) : 0;
+        }
+        ex_next = scales[max(own, 0)];
+        here_next = own >= 0;
+        ask_ids(tile + 1);
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int w = unit(u);
             const int blk = w / D, o = w % D;
             // K: 16 dims of a key; a block that is not there is one of zeros
             const unsigned there = valid[u] > 0 ? ~0u : 0u;
             char* kd = k_lds[buf] + blk * L::kKBlock + (o * 16 / D) * L::kKRow + (o * 16 % D) * 2;
             *(vec8*)kd = C::raw(T{}, kreg[u][0] & there, kreg[u][1] & there);
             *(vec8*)(kd + 16) = C::raw(T{}, kreg[u][2] & there, kreg[u][3] & there);
-            // V: 16 keys of a dim; codes behind the last key count as 0
-            unsigned keep[4];
+            // V: 16 keys of a dim; codes behind the last key have no weight, but a NaN among them would count
+            unsigned keep[4] = {~0u, ~0u, ~0u, ~0u};
+            if (C::kHasNaN) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int in = min(max(valid[u] - 4 * j, 0), 4);
-                keep[j] = in >= 4 ? ~0u : (1u << (8 * in)) - 1u;
+                for (int j = 0; j < 4; ++j) {
+                    const int in = min(max(valid[u] - 4 * j, 0), 4);
+                    keep[j] = in >= 4 ? ~0u : (1u << (8 * in)) - 1u;
+                }
             }
             const unsigned ev = valid[u] > 0 ? ereg[u] >> 8 : 127u;
             char* vd = v_lds[buf] + o * L::kVRow + blk * 16;
@@ -288,28 +271,22 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
         // the next score tile are requested ahead of the products of this one.
         __builtin_amdgcn_s_setprio(2);
         float4v st[COLS][4];
-        vec8 ka[2][kX];
+        constexpr int kNK = 4 * kX;
+        vec8 ka[kVAhead];
+        auto k_operand = [&](int e) { return *(const vec8*)(kl + 4 * (e / kX) * L::kKRow + 64 * (e % kX)); };
+        auto v_operand = [&](int e) { return *(const vec8*)(vl + 16 * (e >> 1) * L::kVRow + 64 * (e & 1)); };
 #pragma unroll
-        for (int x = 0; x < kX; ++x) ka[0][x] = *(const vec8*)(kl + 64 * x);
+        for (int e = 0; e < kVAhead; ++e) ka[e] = k_operand(e);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j < 3) {
+        for (int e = 0; e < kNK; ++e) {
+            const int j = e / kX, x = e % kX;
 #pragma unroll
-                for (int x = 0; x < kX; ++x) ka[(j + 1) & 1][x] = *(const vec8*)(kl + 4 * (j + 1) * L::kKRow + 64 * x);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int u = 0; u < COLS; ++u) st[u][j] = (float4v){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int x = 0; x < kX; ++x)
-#pragma unroll
-                for (int u = 0; u < COLS; ++u) st[u][j] = T::mfma(ka[j & 1][x], qb[u][x], st[u][j]);
+            for (int u = 0; u < COLS; ++u)
+                st[u][j] = T::mfma(ka[e % kVAhead], qb[u][x], x ? st[u][j] : (float4v){0.f, 0.f, 0.f, 0.f});
+            ka[e % kVAhead] = e + kVAhead < kNK ? k_operand(e + kVAhead) : v_operand(e + kVAhead - kNK);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // V operands of the first dim tiles are requested before the softmax, which covers their way
-        vec8 va[kVAhead];
-#pragma unroll
-        for (int e = 0; e < kVAhead; ++e) va[e] = *(const vec8*)(vl + 16 * (e >> 1) * L::kVRow + 64 * (e & 1));
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
         const float f = g.scale2 * pow2_of(here ? ex & 0xffu : 127u);    // > 0: keeps the order of the scores
@@ -328,8 +305,10 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
                     mx = fmaxf(mx, s[e]);
                 }
             } else {
-                mx = max3(max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[8])),
-                          max3(s[9], s[10], s[11]), max3(max3(s[12], s[13], s[14]), s[15], s[15])) * f;
+                mx = s[0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) mx = larger(mx, s[e]);
+                mx *= f;
                 mx = here ? mx : kFar;
             }
             if (__ballot(mx - m_run[u] > kLazyP) != 0) {
@@ -358,19 +337,18 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             lsum[u] = T::mfma(ones, pb[u][1], lsum[u]);
         }
 #pragma unroll
-        for (int t = 0; t < kT; ++t)
+        for (int e = 0; e < 2 * kT; ++e) {
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                const int e = 2 * t + z;
-                const vec8 a = e < kVAhead ? va[e % kVAhead] : *(const vec8*)(vl + 16 * t * L::kVRow + 64 * z);
-#pragma unroll
-                for (int u = 0; u < COLS; ++u) acc[u][t] = T::mfma(a, pb[u][z], acc[u][t]);
-            }
+            for (int u = 0; u < COLS; ++u) acc[u][e >> 1] = T::mfma(ka[e % kVAhead], pb[u][e & 1], acc[u][e >> 1]);
+            if (e + kVAhead < 2 * kT)
+                ka[e % kVAhead] = v_operand(e + kVAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         __builtin_amdgcn_s_setprio(0);
     };
 
     if (tile_begin < tile_end) {
-        load_ids(tile_begin);
+        ask_ids(tile_begin);
         fetch(tile_begin);
         stage(0);
         here = here_next;
@@ -379,15 +357,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     auto iterate = [&](auto masked_tag, int from, int to) {
         for (int tile = from; tile < to; ++tile) {
             const int buf = (tile - tile_begin) & 1;
-            const bool more = tile + 1 < tile_end;
             __syncthreads();                                  // this tile is staged; the other buffer is free
-            if (more) fetch(tile + 1);
+            fetch(tile + 1);                                  // behind the last tile: one more, unused
             if (tile * 64 <= wave_last) consume(masked_tag, buf, tile);
-            if (more) {
-                stage(buf ^ 1);
-                here = here_next;
-                ex = ex_next;
-            }
+            stage(buf ^ 1);
+            here = here_next;
+            ex = ex_next;
         }
     };
     // The tiles that every row of the workgroup sees whole, then those that hold some row's last key.  Two loops, not two
@@ -418,6 +393,40 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             if (c == 0) g.mid_lse[at] = l == 0.f ? kFar : __builtin_amdgcn_logf(l) + m_run[u];
         }
     }
+}
+
+template <class T, class C, int D, int WAVES, int COLS>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn8_prefill_kernel(const Prefill8Args g) {
+    constexpr int kRows = 16 * COLS * WAVES;                  // rows per workgroup
+    __shared__ __attribute__((aligned(16))) char k_lds[2][Lds8<D>::kK];
+    __shared__ __attribute__((aligned(16))) char v_lds[2][Lds8<D>::kV];
+    const int lane = threadIdx.x & 63;
+    // Workgroups are numbered (row tile, split, kv head), the head fastest: consecutive ones go to the eight XCDs in
+    // turn, so that with eight kv heads or a multiple a head's row tiles share one L2.
+    const int Hkv = g.pool.num_kv_heads;
+    const int cell = (int)(blockIdx.x / (unsigned)Hkv);
+    const int kvh = (int)blockIdx.x - cell * Hkv;
+    const int job = cell / g.max_splits;
+    const int split = cell - job * g.max_splits;
+    int b, rank;                                              // rank: the row tile, counted from the chunk's last
+    if (g.sorted) {
+        if (!nth_longest(g, kRows, job, lane, b, rank)) return;
+    } else {
+        rank = job / g.batch.num_prefill_seqs;
+        b = job - rank * g.batch.num_prefill_seqs;
+    }
+    const int64_t start = g.batch.prefill_start_locs[b];
+    const int len = chunk_rows(chunks_of(g.batch), b, start);
+    const int rows = len * g.group;
+    const int tiles = (rows + kRows - 1) / kRows;             // of this chunk
+    if (rank >= tiles) return;
+    const int row0 = (tiles - 1 - rank) * kRows;
+    // A tile that is at most half full: one column tile a wave, on all of them, instead of two on half.  Six chunks of 1 to
+    // 16 tokens of 64 q heads over 8000 to 16000 cached ones: 70 us -> 55.
+    if (COLS == 2 && rows - row0 <= kRows / 2)
+        attend_tile<T, C, D, WAVES, 1>(g, k_lds, v_lds, b, split, kvh, start, rows, row0);
+    else
+        attend_tile<T, C, D, WAVES, COLS>(g, k_lds, v_lds, b, split, kvh, start, rows, row0);
 }
 
 template <class T, class C, int D>
@@ -479,12 +488,12 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     const int64_t columns = (int64_t)pool->num_kv_heads * max_splits * batch->num_prefill_seqs;
     // Rows per workgroup: 64 where a chunk has no more; 256 (one workgroup of eight waves per CU, the conversions of a
     // tile shared by more rows) for long chunks that fill the chip with them -- 2048 x 4 rows over 8192 cached tokens
-    // 425 us against 433 with 128 (int8, bf16: 434 against 464), but 512 rows 53 against 48.
+    // 370 us against 407 with 128, whole prompts of 8192 tokens 637 against 707, but eight of 512 tokens 46 against 42.
     const int shape = rows <= 64 ? 64 : rows > 512 && columns * mkv::cdiv(rows, 256) >= mkv::num_cus() ? 256 : 128;
     const int64_t cells = columns * mkv::cdiv(rows, shape);
     MKV_REQUIRE(cells <= 0x7fffffff, "too many rows in one call");
-    // Finding a workgroup's place in the order costs a few microseconds: 8 x 512 tokens 48 us, sorted 52; four ragged
-    // chunks over up to 7473 cached tokens 1211 us, sorted 676.
+    // Finding a workgroup's place in the order costs a few microseconds: 8 x 512 tokens 42 us, sorted 48; four ragged
+    // chunks over up to 7473 cached tokens 992 us, sorted 605.
     g.key_tiles = mkv::cdiv((int64_t)tokens_per_split * max_splits, 64);
     g.sorted = batch->num_prefill_seqs > 1 && cells > 2 * mkv::num_cus() && g.key_tiles >= 32;
     const dim3 grid((unsigned)cells);

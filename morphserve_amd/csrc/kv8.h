@@ -53,6 +53,7 @@ __device__ __forceinline__ float pow2_of(unsigned biased) { return __builtin_bit
 // float's own bits.  encode4(): four values (already scaled into range) to four codes.  raw(): eight codes to the
 // element type, unscaled; scaled(): times 2^(e - 127).
 struct E4M3 {
+    static constexpr bool kHasNaN = true;
     static __device__ __forceinline__ unsigned exponent(float amax) {       // 448 = 1.75 * 2^8
         const unsigned u = __builtin_bit_cast(unsigned, amax);
         const int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
@@ -89,6 +90,7 @@ struct E4M3 {
 };
 
 struct Int8 {
+    static constexpr bool kHasNaN = false;
     static __device__ __forceinline__ unsigned exponent(float amax) {       // 127 = 1.984375 * 2^6
         const unsigned u = __builtin_bit_cast(unsigned, amax);
         const int e = (int)(u >> 23) - 6 + ((u & 0x7fffffu) > 0x7e0000u);
