@@ -491,7 +491,8 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     // 370 us against 407 with 128, whole prompts of 8192 tokens 637 against 707, but eight of 512 tokens 46 against 42.
     const int shape = rows <= 64 ? 64 : rows > 512 && columns * mkv::cdiv(rows, 256) >= mkv::num_cus() ? 256 : 128;
     const int64_t cells = columns * mkv::cdiv(rows, shape);
-    MKV_REQUIRE(cells <= 0x7fffffff, "too many rows in one call");
+    // a launch holds fewer than 2^32 threads, the joining one up to 256 for every row
+    MKV_REQUIRE(cells * 512 <= 0xffffffffll && (max_splits == 1 || rows * pool->num_kv_heads * 256 <= 0xffffffffll), "too many rows in one call");
     // Finding a workgroup's place in the order costs a few microseconds: 8 x 512 tokens 42 us, sorted 48; four ragged
     // chunks over up to 7473 cached tokens 992 us, sorted 605.
     g.key_tiles = mkv::cdiv((int64_t)tokens_per_split * max_splits, 64);
@@ -503,7 +504,6 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     MKV_HIP(hipGetLastError());
     if (max_splits > 1)
         return mkv::launch_merge8(dtype, pool->head_dim, (const float*)mid_o, (const float*)mid_lse, o, o_stride,
-                                  num_q_heads, dim3((unsigned)(batch->max_prefill_len * num_q_heads), (unsigned)batch->num_prefill_seqs),
-                                  max_splits, mkv::chunks_of(*batch), s);
+                                  num_q_heads, batch->max_prefill_len * num_q_heads, batch->num_prefill_seqs, max_splits, mkv::chunks_of(*batch), s);
     return MKV_OK;
 }

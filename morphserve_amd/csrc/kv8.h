@@ -191,9 +191,9 @@ __host__ __device__ __forceinline__ Chunks8 chunks_of(const mkv_batch& b) {
 }
 
 // Joins the partials of output rows cut into `splits` (mid_o normalised, mid_lse = log2 of the sum of exponentials,
-// kFar where a split held nothing) and writes the rows to o.  grid.x: q heads x rows; grid.y: chunks, where the rows
+// kFar where a split held nothing) and writes the rows to o.  `rows`: q heads x tokens, of the longest chunk where the rows
 // are those of chunks.
 int launch_merge8(int dtype, int head_dim, const float* mid_o, const float* mid_lse, void* o, int64_t o_stride,
-                  int32_t num_q_heads, dim3 grid, int32_t splits, const Chunks8& chunks, hipStream_t s);
+                  int32_t num_q_heads, int32_t rows, int32_t chunk_count, int32_t splits, const Chunks8& chunks, hipStream_t s);
 
 }  // namespace mkv

@@ -69,10 +69,11 @@ def rotary_embedding_and_store_kvcache_8bit(
         infer_state, cur_layer, prefix_lens, q, cos, sin, layout, q_out))
 
 
-def choose_split_8bit(n: int, num_kv_heads: int, max_len: int, target_wgs: int = 512) -> Tuple[int, int]:
-    """``(tokens_per_split, max_splits)`` of a decode launch: enough workgroups for the device (two per compute unit), none
-    with less than a tile of 64 tokens for each of its four waves."""
-    return _capi.binding().decode_split(n, num_kv_heads, max_len, target_wgs)
+def choose_split_8bit(n: int, num_kv_heads: int, max_len: int, units: int = 256, num_q_heads: Optional[int] = None,
+                      head_dim: int = 128) -> Tuple[int, int]:
+    """``(tokens_per_split, max_splits)`` of a decode launch over ``n`` rows on ``units`` compute units: the ranges with the
+    least estimated time, their joining included."""
+    return _capi.binding().decode_split(n, num_kv_heads, max_len, units, num_q_heads or num_kv_heads, head_dim)
 
 
 def paged_attention_8bit(
@@ -93,10 +94,9 @@ def paged_attention_8bit(
 
 
 def choose_prefill_split_8bit(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_len: int, max_keys: int,
-                              target_wgs: int = 512) -> Tuple[int, int]:
-    """``(tokens_per_split, max_splits)`` of a chunk launch: the keys are cut only where the row tiles alone leave
-    compute units idle, into ranges of at least four tiles."""
-    return _capi.binding().prefill_split(num_seqs, num_q_heads, num_kv_heads, max_len, max_keys, target_wgs)
+                              units: int = 256, head_dim: int = 128) -> Tuple[int, int]:
+    """``(tokens_per_split, max_splits)`` of a chunk launch, chosen like a decode launch's."""
+    return _capi.binding().prefill_split(num_seqs, num_q_heads, num_kv_heads, max_len, max_keys, units, head_dim)
 
 
 def chunked_prefill_attention_8bit(

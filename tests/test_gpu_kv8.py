@@ -287,6 +287,16 @@ def test_chunks_split_over_the_keys(cuda, monkeypatch, dtype, kind, splits):
     assert_within(prefill(b, cuda, q), *b.expect_chunks(q))
 
 
+@pytest.mark.parametrize("splits", [4, 5, 8, 9])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_rows_split_over_the_keys(cuda, monkeypatch, dim, splits):
+    """Partials joined by a wave a row and by four, ranges without a key among them."""
+    b = Batch(36, hq=16, hkv=4, dim=dim, dtype="bf16", chunks=[140, 3, 0, 131], prefixes=[100, 260, 30, 0])
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
+    q = b.new_rows(b.hq)
+    assert_within(prefill(b, cuda, q), *b.expect_chunks(q))
+
+
 @pytest.mark.parametrize("hint", [True, False])
 @pytest.mark.parametrize("seqs", [2, 70])
 def test_row_tiles_in_order_of_length(cuda, seqs, hint):
