@@ -445,8 +445,8 @@ typedef struct mkv_pool8 {
 /* The rows of one step, prefill sequences first: rows prefill_start_locs[b] + t,
  * t < prefill_lens[b], hold positions prefix_lens[b] + t of sequence seq_ids[b]; row
  * num_prefill_tokens + i holds position decoding_lens[i] - 1 of sequence
- * seq_ids[num_prefill_seqs + i].  prefix_lens NULL = 0.  max_prefill_len bounds
- * prefill_lens on the host.  A sequence appears once in a batch.  A sequence id
+ * seq_ids[num_prefill_seqs + i].  prefix_lens NULL = 0, as a
+ * negative one counts.  max_prefill_len bounds prefill_lens on the host.  A sequence appears once in a batch.  A sequence id
  * outside the table, a table entry that names no block of the pool and positions
  * beyond the table row hold nothing: they are neither read nor written. */
 typedef struct mkv_batch {
@@ -497,7 +497,9 @@ int mkv_store8(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, con
  * nothing to attend to (length 0, or none of its blocks in the pool) gets zeros.
  * tokens_per_split (a multiple of 64) and max_splits as there; mid_o (fp32
  * [n, Hq, max_splits, D], 16-byte aligned) and mid_lse (fp32 [n, Hq, max_splits])
- * may be NULL when max_splits is 1. */
+ * may be NULL when max_splits is 1.  At most 65535 rows; tokens_per_split times
+ * max_splits at most 2^33.  Sums are held in 32 bits with weights up to 2^8: values
+ * of V beyond 2^119 (bf16) may overflow them. */
 int mkv_attn8_decode(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* q,
                      void* o, int64_t q_stride, int64_t o_stride, int32_t num_q_heads,
                      float softmax_scale, int32_t layer, int32_t tokens_per_split,
@@ -509,7 +511,10 @@ int mkv_attn8_decode(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtyp
  * sequence are cut into max_splits ranges of tokens_per_split (a multiple of 64; the
  * last range takes whatever lies behind it); with max_splits > 1 the partials go
  * through mid_o (fp32 [num_prefill_tokens, Hq, max_splits, D]) and mid_lse (fp32
- * [num_prefill_tokens, Hq, max_splits]). */
+ * [num_prefill_tokens, Hq, max_splits]).  softmax_scale must be positive.
+ * A NaN in V spoils the rows that see its key, and may spoil earlier rows of the same
+ * chunk whose own last key is among the same 64 (its weight there is 0, and 0 times
+ * NaN is NaN); other sequences' rows never. */
 int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* q,
                       void* o, int64_t q_stride, int64_t o_stride, int32_t num_q_heads,
                       float softmax_scale, int32_t layer, int32_t tokens_per_split,

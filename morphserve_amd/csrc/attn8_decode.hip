@@ -322,7 +322,6 @@ __global__ __launch_bounds__(256) void merge8_few_kernel(const float* __restrict
     typedef typename T::elem E;
     constexpr int kDims = D / 64;
     typedef float vecd __attribute__((ext_vector_type(kDims)));
-    typedef E vece __attribute__((ext_vector_type(kDims)));
     const int lane = threadIdx.x & 63;
     const int row = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (row >= rows) return;
@@ -412,6 +411,8 @@ extern "C" int mkv_attn8_decode(const mkv_pool8* pool, const mkv_batch* batch, i
     MKV_REQUIRE(tokens_per_split > 0 && tokens_per_split % 64 == 0, "tokens_per_split %d must be a positive multiple of 64",
                 tokens_per_split);
     MKV_REQUIRE(max_splits >= 1, "max_splits must be >= 1");
+    // tile and block numbers, those behind the last key included, are 32-bit
+    MKV_REQUIRE((int64_t)tokens_per_split * max_splits <= (int64_t)1 << 33, "%d ranges of %d tokens are too long", max_splits, tokens_per_split);
     MKV_REQUIRE(max_splits == 1 || (mid_o && mid_lse), "scratch buffers are NULL");
     MKV_REQUIRE(((uintptr_t)mid_o & 15) == 0 && ((uintptr_t)mid_lse & 3) == 0, "mid_o must be 16-byte aligned, mid_lse 4-byte aligned");
     MKV_REQUIRE(((uintptr_t)q & 15) == 0 && (q_stride & 7) == 0, "q rows must be 16-byte aligned");

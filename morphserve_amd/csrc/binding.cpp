@@ -127,11 +127,25 @@ const int32_t* ints_of(const at::Tensor& t, const char* what, const at::Tensor& 
     return (const int32_t*)t.const_data_ptr();
 }
 
-const int32_t* int_tensor_attr(PyObject* o, PyObject* name, const at::Tensor& like, int64_t least) {
-    Attr a(o, name);
-    const char* what = PyUnicode_AsUTF8(name);
-    return ints_of(tensor(a.value, what), what, like, least);       // the state object keeps the tensor
-}
+// The tensors of a state object, kept until the launch is out: one whose attributes are made anew at every access must not
+// see its memory handed to the call's own scratch.
+struct Held {
+    PyObject* objects[8];
+    int count = 0;
+    Held() = default;
+    Held(const Held&) = delete;
+    Held& operator=(const Held&) = delete;
+    ~Held() {
+        while (count > 0) Py_DECREF(objects[--count]);
+    }
+    const int32_t* ints(PyObject* o, PyObject* name, const at::Tensor& like, int64_t least) {
+        PyObject* value = PyObject_GetAttr(o, name);
+        if (!value) throw Refused{};
+        objects[count++] = value;
+        const char* what = PyUnicode_AsUTF8(name);
+        return ints_of(tensor(value, what), what, like, least);
+    }
+};
 
 // Makes the rows' device current for a call, where it is not; its current stream.
 struct OnDevice {
@@ -195,7 +209,7 @@ mkv_pool8 pool_for(PyObject* const* cache, PyObject* model, PyObject* engine, co
 }
 
 // The step's prefill rows, decode rows or both.
-mkv_batch batch_of(const at::Tensor& table, PyObject* st, const at::Tensor& like, bool prefill, bool decode, PyObject* prefix_lens) {
+mkv_batch batch_of(const at::Tensor& table, PyObject* st, const at::Tensor& like, bool prefill, bool decode, PyObject* prefix_lens, Held& held) {
     if (table.dim() != 2) refuse("block_table must be [max_seqs, max_blocks_per_seq]");
     mkv_batch b = {};
     b.block_table = ints_of(table, "block_table", like, 0);
@@ -210,13 +224,13 @@ mkv_batch batch_of(const at::Tensor& table, PyObject* st, const at::Tensor& like
     }
     if (decode) b.num_decoding_seqs = int_attr(st, names.num_decoding_seqs);
     const int32_t skipped = prefill ? 0 : seqs;
-    b.seq_ids = int_tensor_attr(st, names.seq_ids, like, (int64_t)skipped + b.num_prefill_seqs + std::max(b.num_decoding_seqs, 0)) + skipped;
+    b.seq_ids = held.ints(st, names.seq_ids, like, (int64_t)skipped + b.num_prefill_seqs + std::max(b.num_decoding_seqs, 0)) + skipped;
     if (b.num_prefill_seqs) {
-        b.prefill_start_locs = int_tensor_attr(st, names.prefill_seq_start_locs, like, b.num_prefill_seqs);
-        b.prefill_lens = int_tensor_attr(st, names.prefill_seq_lens, like, b.num_prefill_seqs);
+        b.prefill_start_locs = held.ints(st, names.prefill_seq_start_locs, like, b.num_prefill_seqs);
+        b.prefill_lens = held.ints(st, names.prefill_seq_lens, like, b.num_prefill_seqs);
         if (prefix_lens != Py_None) b.prefix_lens = ints_of(tensor(prefix_lens, "prefix_lens"), "prefix_lens", like, b.num_prefill_seqs);
     }
-    if (b.num_decoding_seqs > 0) b.decoding_lens = int_tensor_attr(st, names.decoding_seq_lens, like, b.num_decoding_seqs);
+    if (b.num_decoding_seqs > 0) b.decoding_lens = held.ints(st, names.decoding_seq_lens, like, b.num_decoding_seqs);
     return b;
 }
 
@@ -385,7 +399,8 @@ int store(PyObject* const* a, Py_ssize_t count) {
     const int32_t dtype = dtype_of(k, "k");
     on_gpu(k, "k");
     const mkv_pool8 p = pool_for(a + 3, a[7], a[8], k);
-    const mkv_batch b = batch_of(tensor(a[6], "block_table"), a[9], k, true, true, a[11]);
+    Held held;
+    const mkv_batch b = batch_of(tensor(a[6], "block_table"), a[9], k, true, true, a[11], held);
     const int64_t tokens = (int64_t)b.num_prefill_tokens + b.num_decoding_seqs;
     const int64_t ks = rows_of(k, "k", k, tokens, p.num_kv_heads, p.head_dim), vs = rows_of(v, "v", k, tokens, p.num_kv_heads, p.head_dim);
     const int32_t layer = small(a[10], "cur_layer");
@@ -413,7 +428,8 @@ int decode(PyObject* const* a, Py_ssize_t count) {
     const int32_t dtype = dtype_of(q, "q");
     on_gpu(q, "q");
     const mkv_pool8 p = pool_for(a + 2, a[6], a[7], q);
-    const mkv_batch b = batch_of(tensor(a[5], "block_table"), a[8], q, false, true, Py_None);
+    Held held;
+    const mkv_batch b = batch_of(tensor(a[5], "block_table"), a[8], q, false, true, Py_None, held);
     const int32_t n = b.num_decoding_seqs, heads = int_attr(a[6], names.num_q_heads);
     const int64_t qs = rows_of(q, "q", q, n, heads, p.head_dim), os = out_rows_of(o, "o", q, n, heads, p.head_dim);
     const int32_t layer = small(a[9], "cur_layer");
@@ -438,7 +454,8 @@ int prefill(PyObject* const* a, Py_ssize_t count) {
     const int32_t dtype = dtype_of(q, "q");
     on_gpu(q, "q");
     const mkv_pool8 p = pool_for(a + 2, a[6], a[7], q);
-    const mkv_batch b = batch_of(tensor(a[5], "block_table"), a[8], q, true, false, a[11]);
+    Held held;
+    const mkv_batch b = batch_of(tensor(a[5], "block_table"), a[8], q, true, false, a[11], held);
     const int32_t tokens = b.num_prefill_tokens, heads = int_attr(a[6], names.num_q_heads);
     const int64_t qs = rows_of(q, "q", q, tokens, heads, p.head_dim), os = out_rows_of(o, "o", q, tokens, heads, p.head_dim);
     const int32_t layer = small(a[9], "cur_layer");

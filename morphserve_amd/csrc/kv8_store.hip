@@ -49,8 +49,8 @@ __device__ __forceinline__ bool find_cell(const Store8Args& g, int cell, Cell& c
         const int j = cell - m.num_decoding_seqs - s * g.blocks_per_seq;
         const int64_t start = m.prefill_start_locs[s];
         const int64_t len = chunk_rows(chunks_of(m), s, start);
-        const int64_t prefix = m.prefix_lens ? m.prefix_lens[s] : 0;
-        if (len <= 0 || prefix < 0) return false;
+        const int64_t prefix = m.prefix_lens ? max(m.prefix_lens[s], 0) : 0;
+        if (len <= 0) return false;
         blk = prefix / kBlk + j;
         const int64_t first = max(prefix, blk * kBlk), end = min(prefix + len, (blk + 1) * kBlk);
         if (first >= end) return false;
@@ -436,7 +436,7 @@ int mkv_store8(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, con
     g.blocks_per_seq = prefill ? mkv::cdiv(batch->max_prefill_len, mkv::kBlk) + (batch->prefix_lens ? 1 : 0) : 0;
     const int64_t cells = (int64_t)batch->num_prefill_seqs * g.blocks_per_seq + batch->num_decoding_seqs;
     g.unit_groups = mkv::cdiv(units, 4);
-    MKV_REQUIRE(cells * g.unit_groups <= 0x7fffffff, "too many rows in one call");
+    MKV_REQUIRE(cells * g.unit_groups * 256 <= 0xffffffffll, "too many rows in one call");      // threads of a launch
     const dim3 grid((unsigned)(cells * g.unit_groups));
     hipStream_t s = (hipStream_t)stream;
     const bool rot = rope != MKV_ROPE_NONE;

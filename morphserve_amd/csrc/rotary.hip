@@ -107,6 +107,8 @@ extern "C" int mkv_rope_positions(int32_t dtype, int32_t layout, const void* q, 
     const int64_t q_row = (int64_t)num_q_heads * head_dim, k_row = (int64_t)num_kv_heads * head_dim;
     MKV_REQUIRE(num_tokens == 1 || (q_stride >= q_row && q_out_stride >= q_row && k_stride >= k_row && k_out_stride >= k_row),
                 "rows overlap: a stride is shorter than its row");
+    MKV_REQUIRE(num_tokens == 1 || ((q != q_out || q_stride == q_out_stride) && (!k || k != k_out || k_stride == k_out_stride)),
+                "in place, input and output have one stride");
     // as many pairs to a thread as the row cuts into and the addresses are aligned for
     uintptr_t at = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out;
     int64_t strides = q_stride | q_out_stride;

@@ -454,6 +454,41 @@ def test_calls_on_two_streams_at_once(cuda):
         assert torch.equal(o, outs[0])
 
 
+def test_state_whose_tensors_are_made_at_every_access(cuda, monkeypatch):
+    """The call's scratch must not take the memory of a tensor that only the call still holds."""
+    b = Batch(45, hq=8, hkv=2, chunks=[70, 9], prefixes=[100, 0], dec=[3000, 2500, 64])
+    kept = b.state(cuda)
+
+    class State:
+        def __getattr__(self, name):
+            value = getattr(kept, name)
+            return value.clone() if isinstance(value, torch.Tensor) else value
+
+    monkeypatch.setattr(b, "state", lambda device: State())
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, 2))       # partials of a few hundred bytes and more
+    q = b.new_rows(b.hq)
+    n = sum(b.chunks)
+    want, bound = b.expect_decode(q[n:])
+    assert_within(decode(b, cuda, q[n:]), want, bound)
+    assert_within(prefill(b, cuda, q[:n]), *b.expect_chunks(q[:n]))
+
+
+def test_negative_prefixes_count_as_none(cuda):
+    b = Batch(46, hq=4, hkv=2, chunks=[20, 40], prefixes=[0, 0])
+    q = b.new_rows(b.hq)
+    want = prefill(b, cuda, q)
+    b.prefixes = [-1, -(2 ** 31)]
+    assert torch.equal(prefill(b, cuda, q, hint=False), want)
+    results = []
+    for prefixes in ([0, 0], b.prefixes):
+        b.prefixes = prefixes
+        cache, st = b.cache(cuda), b.state(cuda)
+        k = rounded(q[:, :2], "f16").to(cuda)
+        store_kvcache_8bit(k, k, cache, b.block_table(cuda), b.model, b.engine, st, b.layer, prefix_lens=b.prefix_tensor(cuda))
+        results.append([cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.scales])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
 def test_empty_calls(cuda):
     b = Batch(43, chunks=[], dec=[])
     st, cache, table = b.state(cuda), b.cache(cuda), torch.full((3, 2), -1, dtype=torch.int32, device=cuda)

@@ -203,9 +203,27 @@ def test_bad_attention(entry, bad):
     assert attn(entry, **bad) == _capi.MKV_EINVAL
 
 
+@pytest.mark.parametrize("entry", ["mkv_attn8_decode", "mkv_attn8_prefill"])
+@pytest.mark.parametrize("tps,splits", [(2 ** 30, 16), (2 ** 31 - 64, 5), (2 ** 20, 2 ** 14), (64, 2 ** 28)])
+def test_ranges_whose_ends_have_no_32_bit_number(entry, tps, splits):
+    assert attn(entry, tps=tps, splits=splits) == _capi.MKV_EINVAL
+    assert b"ranges" in _capi.lib().mkv_last_error()
+
+
+def test_launches_too_large():
+    """2^32 threads and more in one launch."""
+    many = dict(num_prefill_seqs=2000, max_prefill_len=2 ** 17)
+    assert store(b=batch8(**many)) == _capi.MKV_EINVAL and b"too many rows" in _capi.lib().mkv_last_error()
+    assert attn("mkv_attn8_prefill", b=batch8(num_prefill_seqs=60000, max_prefill_len=2 ** 20)) == _capi.MKV_EINVAL
+    assert b"too many rows" in _capi.lib().mkv_last_error()
+    assert attn("mkv_attn8_prefill", b=batch8(num_prefill_seqs=1, max_prefill_len=2 ** 22)) == _capi.MKV_EINVAL
+    assert attn("mkv_attn8_decode", b=batch8(num_decoding_seqs=65536)) == _capi.MKV_EINVAL
+    assert attn("mkv_attn8_decode", p=pool8(num_kv_heads=64), hq=1024, b=batch8(num_decoding_seqs=40000)) == _capi.MKV_EINVAL
+
+
 @pytest.mark.parametrize("bad", [dict(dtype=5), dict(layout=0), dict(layout=3), dict(tokens=-1), dict(hq=0), dict(hkv=-1), dict(rotary=7),
                                  dict(rotary=0), dict(rotary=66), dict(q=None), dict(k=None), dict(pos=None), dict(cos=None),
-                                 dict(positions=-1), dict(qs=100), dict(dim=0)])
+                                 dict(positions=-1), dict(qs=100), dict(dim=0), dict(qos=512), dict(kos=256)])
 def test_bad_rotary(bad):
     a = dict(dtype=0, layout=1, q=A, k=A, qo=A, ko=A, qs=256, ks=128, qos=256, kos=128, pos=A, cos=A, sin=A, positions=9, tokens=3,
              hq=4, hkv=2, dim=64, rotary=32)
