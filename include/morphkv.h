@@ -511,10 +511,8 @@ int mkv_attn8_decode(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtyp
  * sequence are cut into max_splits ranges of tokens_per_split (a multiple of 64; the
  * last range takes whatever lies behind it); with max_splits > 1 the partials go
  * through mid_o (fp32 [num_prefill_tokens, Hq, max_splits, D]) and mid_lse (fp32
- * [num_prefill_tokens, Hq, max_splits]).  softmax_scale must be positive.
- * A NaN in V spoils the rows that see its key, and may spoil earlier rows of the same
- * chunk whose own last key is among the same 64 (its weight there is 0, and 0 times
- * NaN is NaN); other sequences' rows never. */
+ * [num_prefill_tokens, Hq, max_splits]).  softmax_scale must be positive.  A NaN among
+ * the keys is in the sums of the rows at and behind its position and in no other's. */
 int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* q,
                       void* o, int64_t q_stride, int64_t o_stride, int32_t num_q_heads,
                       float softmax_scale, int32_t layer, int32_t tokens_per_split,

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
 }
 
 // One workgroup per output row -- of a prefill chunk (blockIdx.y) or, without start_locs, of the decode batch; wave w
-// takes the partials w, w + 4, ... of the row.  A partial that holds nothing (its log sum at kFar) weighs nothing.
+// takes the partials w, w + 4, ... of the row.  A partial that holds nothing (its log sum at kFar) weighs nothing; one whose sum is a NaN counts.
 template <class T, int D>
 __global__ __launch_bounds__(256) void merge8_kernel(const float* __restrict__ mid_o, const float* __restrict__ mid_lse,
                                                      char* __restrict__ o, int64_t o_stride, int32_t num_q_heads,
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256) void merge8_kernel(const float* __restrict__ m
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (s0 + 4 * e < splits && w[e] > 0.5f * kFar) {
+            if (s0 + 4 * e < splits && !(w[e] <= 0.5f * kFar)) {
                 const float f = __builtin_amdgcn_exp2f(w[e] - m);
                 l += f;
                 a += f * v[e];
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256) void merge8_few_kernel(const float* __restrict
     vecd a = (vecd)0.f;
 #pragma unroll
     for (int s = 0; s < kFewSplits; ++s) {
-        if (s < splits && w[s] > 0.5f * kFar) {
+        if (s < splits && !(w[s] <= 0.5f * kFar)) {
             const float f = __builtin_amdgcn_exp2f(w[s] - m);
             l += f;
             a += f * v[s];

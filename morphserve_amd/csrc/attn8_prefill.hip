@@ -55,6 +55,18 @@ struct Lds8 {
     static constexpr int kV = D * kVRow;
 };
 
+// A row does not see every key of its last tiles, and a NaN there must not reach it through a weight of 0: where such tiles
+// are staged, V's NaN are taken out and noted, a bit for each key and dim, and put into the rows that see their keys.  Costs
+// 2 % on long prompts (e4m3; int8 has no NaN).
+template <int D>
+struct NaN8 {
+    uint64_t keys[2][D];                      // of the staged tiles: dim's keys 0 .. 63 with a NaN
+    union {
+        uint8_t wave[2][8];                   // has the wave met one among the units that it staged
+        uint64_t any[2];
+    };
+};
+
 // Which row tile is the job-th longest of the batch?  A launch that does not fit the chip at once is as long as its last
 // workgroups make it, so the row tiles with most keys go first, whatever chunk they belong to.  A chunk's tiles with at
 // least t key tiles are its last ones and their number has a closed form; the t that the job falls on is found by
@@ -131,7 +143,7 @@ __device__ __forceinline__ bool nth_longest(const Prefill8Args& g, int per, int 
 
 // A workgroup's row tile against its range of the keys: rows row0 .. of the `rows` of chunk b, starting at batch row `start`.
 template <class T, class C, int D, int WAVES, int COLS>
-__device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)[Lds8<D>::kK], char (*v_lds)[Lds8<D>::kV], int b,
+__device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)[Lds8<D>::kK], char (*v_lds)[Lds8<D>::kV], NaN8<D>& nans, int b,
                                             int split, int kvh, int64_t start, int rows, int row0) {
     typedef typename T::elem E;
     typedef typename T::vec8 vec8;
@@ -233,7 +245,10 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
         here_next = own >= 0;
         ask_ids(tile + 1);
     };
-    auto stage = [&](int buf) {
+    // The tiles that every row of the workgroup sees whole end here.
+    const int full_end = max(tile_begin, min(tile_end, (int)((min(prefix + row0 / G, room - 1) + 1) >> 6)));
+    auto stage = [&](int buf, int tile) {
+        unsigned found = 0;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int w = unit(u);
@@ -252,10 +267,26 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
                     keep[j] = in >= 4 ? ~0u : (1u << (8 * in)) - 1u;
                 }
             }
+            if (C::kHasNaN && tile >= full_end) {
+                unsigned keys = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    // a byte's top bit where its code is a NaN: all seven bits below are set
+                    const unsigned at = (((vreg[u][j] & keep[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                    keep[j] &= ~(at * 0xffu);
+                    keys |= ((at * 0x01020408u) >> 24 & 0xfu) << (4 * j);
+                }
+                ((uint16_t*)&nans.keys[buf][o])[blk] = (uint16_t)keys;
+                found |= keys;
+            }
             const unsigned ev = valid[u] > 0 ? ereg[u] >> 8 : 127u;
             char* vd = v_lds[buf] + o * L::kVRow + blk * 16;
             *(vec8*)vd = C::scaled(T{}, vreg[u][0] & keep[0], vreg[u][1] & keep[1], ev);
             *(vec8*)(vd + 64) = C::scaled(T{}, vreg[u][2] & keep[2], vreg[u][3] & keep[3], ev);
+        }
+        if (C::kHasNaN && tile >= full_end) {
+            const bool some = __ballot(found != 0) != 0;
+            nans.wave[buf][wave] = some;
         }
     };
 
@@ -345,12 +376,27 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
+        const auto any = WAVES == 8 ? nans.any[buf] : (uint64_t)*(const uint32_t*)nans.wave[buf];
+        if (C::kHasNaN && MASKED && __ballot(any != 0) != 0) {
+#pragma unroll
+            for (int u = 0; u < COLS; ++u) {
+                const int upto = last_key[u] - 64 * tile + 1;
+                const uint64_t seen = upto <= 0 ? 0 : upto >= 64 ? ~0ull : (1ull << upto) - 1;
+#pragma unroll
+                for (int t = 0; t < kT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {                    // a NaN or 0 is added
+                        const uint64_t hit = nans.keys[buf][16 * t + 4 * c + e] & seen;
+                        acc[u][t][e] += __builtin_bit_cast(float, min((unsigned)hit | (unsigned)(hit >> 32), 1u) * 0x7fc00000u);
+                    }
+            }
+        }
     };
 
     if (tile_begin < tile_end) {
         ask_ids(tile_begin);
         fetch(tile_begin);
-        stage(0);
+        stage(0, tile_begin);
         here = here_next;
         ex = ex_next;
     }
@@ -360,14 +406,13 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
             __syncthreads();                                  // this tile is staged; the other buffer is free
             fetch(tile + 1);                                  // behind the last tile: one more, unused
             if (tile * 64 <= wave_last) consume(masked_tag, buf, tile);
-            stage(buf ^ 1);
+            stage(buf ^ 1, tile + 1);
             here = here_next;
             ex = ex_next;
         }
     };
     // The tiles that every row of the workgroup sees whole, then those that hold some row's last key.  Two loops, not two
     // bodies in one: the accumulators would be copied where the bodies meet, and the registers do not suffice for that.
-    const int full_end = max(tile_begin, min(tile_end, (int)((min(prefix + row0 / G, room - 1) + 1) >> 6)));
     iterate(std::false_type{}, tile_begin, full_end);
     iterate(std::true_type{}, full_end, tile_end);
 
@@ -400,6 +445,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     constexpr int kRows = 16 * COLS * WAVES;                  // rows per workgroup
     __shared__ __attribute__((aligned(16))) char k_lds[2][Lds8<D>::kK];
     __shared__ __attribute__((aligned(16))) char v_lds[2][Lds8<D>::kV];
+    __shared__ NaN8<D> nans;
     const int lane = threadIdx.x & 63;
     // Workgroups are numbered (row tile, split, kv head), the head fastest: consecutive ones go to the eight XCDs in
     // turn, so that with eight kv heads or a multiple a head's row tiles share one L2.
@@ -424,9 +470,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     // A tile that is at most half full: one column tile a wave, on all of them, instead of two on half.  Six chunks of 1 to
     // 16 tokens of 64 q heads over 8000 to 16000 cached ones: 70 us -> 55.
     if (COLS == 2 && rows - row0 <= kRows / 2)
-        attend_tile<T, C, D, WAVES, 1>(g, k_lds, v_lds, b, split, kvh, start, rows, row0);
+        attend_tile<T, C, D, WAVES, 1>(g, k_lds, v_lds, nans, b, split, kvh, start, rows, row0);
     else
-        attend_tile<T, C, D, WAVES, COLS>(g, k_lds, v_lds, b, split, kvh, start, rows, row0);
+        attend_tile<T, C, D, WAVES, COLS>(g, k_lds, v_lds, nans, b, split, kvh, start, rows, row0);
 }
 
 template <class T, class C, int D>

@@ -331,6 +331,45 @@ def test_chunks_with_missing_blocks(cuda):
         assert not o[40:60].any() and not o[90:].any()
 
 
+@pytest.mark.parametrize("which", ["k", "v", "both"])
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("dtype,dim,hq", [("f16", 128, 4), ("bf16", 128, 16), ("f16", 64, 32), ("bf16", 64, 2)])
+def test_nan_reaches_the_rows_that_see_its_key(cuda, monkeypatch, dtype, dim, hq, splits, which):
+    """A NaN among the keys is in the sums of the rows at and behind its position, and in no other's: not through a weight of
+    0 either.  K's spoils a row's whole head, V's the head dims that hold one."""
+    b = Batch(37, hq=hq, hkv=2, dim=dim, dtype=dtype, chunks=[150, 20, 64, 5, 130], prefixes=[70, 3, 0, 300, 0], dec=[90, 40])
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
+    q = b.new_rows(hq)
+    n, group = sum(b.chunks), hq // 2
+    first = b.prefixes + [0, 0]
+    #       sequence, position, head, dim
+    plant = [(0, 10, 0, 3), (0, 100, 1, 5), (0, 219, 0, dim - 1), (0, 130, 0, 17), (1, 12, 0, 0), (2, 63, 1, 7), (2, 1, 0, 9),
+             (3, 304, 1, 33), (4, 64, 1, 2), (4, 65, 1, 2), (4, 127, 0, 50), (5, 89, 0, 1), (5, 20, 0, 21), (6, 39, 1, 4)]
+    spoiled = np.zeros((b.tokens, hq, dim), dtype=bool)
+    codes = []
+    for i, (s, pos, h, d) in enumerate(plant):
+        in_k = which == "k" or (which == "both" and i % 3 == 0)
+        pid = b.table[b.seq_ids[s], pos // 16]
+        at = (b.kc, (pid, b.layer, h, pos % 16, d)) if in_k else (b.vc, (pid, b.layer, h, d, pos % 16))
+        at[0][at[1]] = 0                                    # the rows that do not see it do not care
+        codes.append((at, 0x7f if i % 2 else 0xff))
+        heads, dims = slice(h * group, (h + 1) * group), slice(None) if in_k else d
+        if s < len(b.chunks):
+            row0 = int(b.starts[s]) + max(pos - first[s], 0)
+            spoiled[row0:int(b.starts[s]) + b.chunks[s], heads, dims] = True
+        else:
+            spoiled[n + s - len(b.chunks), heads, dims] = True
+    want, bound = b.expect_chunks(q[:n])
+    want_d, bound_d = b.expect_decode(q[n:])
+    for (array, at), code in codes:
+        array[at] = code
+    got = torch.cat([prefill(b, cuda, q[:n]), decode(b, cuda, q[n:]).view(-1, hq, dim)])
+    assert np.array_equal(torch.isnan(got).cpu().numpy(), spoiled)
+    got[torch.from_numpy(spoiled).to(cuda)] = 0
+    want, bound = np.concatenate([want, want_d]), np.concatenate([bound, bound_d])
+    assert_within(got, np.where(spoiled, 0, want), np.where(spoiled, 1, bound))
+
+
 @pytest.mark.parametrize("splits", [1, 3])
 def test_rows_of_no_chunk_stay(cuda, monkeypatch, splits):
     """Rows between and behind the chunks are neither read nor written."""
