@@ -12,6 +12,12 @@
 // accumulators of a lane are the sixteen scores of ONE block in token order -- K's scale is one factor per lane --
 // and, rounded, they are the second product's operand in the order in which V's sixteen bytes per head dim lie.
 // The running maximum moves only when some score has outgrown it by kLazy octaves.
+//
+// Bound: reading the codes.  64 rows of 1024 to 1536 tokens, 8 kv heads x 128: 32.4 us, 5.2 TB/s; the same loads without any
+// work 27.9 us.  128 rows and 64 q heads (int8, bf16) 61.6 us, 5.5 TB/s; 5 rows of up to 60000 tokens 96.8 us, 5.3 TB/s with
+// the join.  Codes of a wave's next tile are asked for as soon as their registers are free, K's between the two products and
+// V's behind the second; what remains is that a wave waits for its K with its V in flight.  A third wave per SIMD, loads in
+// pieces as single registers become free, and loads that the caches keep were no faster.
 #include <type_traits>
 
 #include "kv8.h"

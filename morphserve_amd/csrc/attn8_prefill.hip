@@ -12,9 +12,9 @@
 // per lane and the scores, exponentiated, the operand of the second product.  V arrives transposed from the cache,
 // so that both products read LDS in rows.  Where few rows meet many keys, the keys are cut into splits.
 //
-// Bound: the matrix cores where rows are many -- 2048 tokens of 32 q heads after 8192 cached ones take 370 us, 835 TFLOP/s
-// of the two products, whole prompts of 8192 tokens 623 us (882) -- less what the softmax leaves them idle: the two waves of
-// a SIMD alternate between products and exponentials.  A wave reads its operands from LDS four ahead of the products, K's
+// Bound: the matrix cores where rows are many -- 2048 tokens of 32 q heads after 8192 cached ones take 365 to 380 us, 815 to
+// 850 TFLOP/s of the two products, whole prompts of 8192 tokens 605 to 650 us (830 to 900) -- less what the softmax leaves
+// them idle: the two waves of a SIMD alternate between products and exponentials.  A wave reads its operands from LDS four ahead of the products, K's
 // last ones already V's first, and nothing is loaded under a condition, since waits where two paths meet take the worse one.
 #include <type_traits>
 

@@ -6,7 +6,8 @@
 // and written once.  A thread takes VEC pairs of one head (16 bytes of each member of the pair for VEC = 8) or,
 // where the output is another tensor, VEC of the dims behind the rotated ones.  The tokens' units are numbered
 // through, so that a workgroup is full whatever the number of heads; a token's table row is read by its heads from
-// the caches.
+// the caches.  16385 tokens of 32 + 8 heads x 128, half of each head rotated, into other tensors: 77.6 us for 340 MB, 4.4 TB/s; 64 tokens
+// 3.9 us, the launch.
 #include "kv8.h"
 
 namespace mkv {
