@@ -66,8 +66,9 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
     const int Hq = g.pool.num_kv_heads * G;
 
     const int64_t seq = g.batch.seq_ids[g.batch.num_prefill_seqs + i];
+    const int known_len = max(g.batch.decoding_lens[i], 0);      // asked for with the sequence, not behind it
     const bool has_row = seq >= 0 && seq < g.batch.table_rows;
-    const int len = has_row ? (int)min((int64_t)max(g.batch.decoding_lens[i], 0), g.batch.max_blocks_per_seq * kBlk) : 0;
+    const int len = has_row ? (int)min((int64_t)known_len, g.batch.max_blocks_per_seq * kBlk) : 0;
     const int32_t* table = g.batch.block_table + (has_row ? seq * g.batch.max_blocks_per_seq : 0);
     const int nblk = (len + kBlk - 1) / kBlk;
     const int num_tiles = (len + 63) >> 6;
