@@ -332,7 +332,7 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
                 mx = kFar;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    s[e] = e < seen ? s[e] * f : kFar;
+                    s[e] = e < seen ? s[e] * f : 2 * kFar;            // so far below that it weighs 0 whatever the maximum
                     mx = fmaxf(mx, s[e]);
                 }
             } else {
@@ -353,7 +353,7 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
             const float off = here ? -m_run[u] : kFar;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                if (MASKED) s[e] = e < seen ? __builtin_amdgcn_exp2f(s[e] - m_run[u]) : 0.f;
+                if (MASKED) s[e] = __builtin_amdgcn_exp2f(s[e] - m_run[u]);
                 else s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], f, off));
             }
 #pragma unroll

@@ -310,6 +310,18 @@ def test_row_tiles_in_order_of_length(cuda, seqs, hint):
     assert_within(prefill(b, cuda, q, hint=hint), *b.expect_chunks(q))
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("heads,chunks", [(16, "short"), (64, [600, 513, 257])])
+def test_several_rounds_of_row_tiles(cuda, heads, chunks, kind):
+    """Enough row tiles for several rounds of workgroups, of chunks with one to five of them; prefixes that end inside a block."""
+    rng = np.random.default_rng(38)
+    chunks = [int(x) for x in rng.integers(0, 200, 40)] + [300, 129, 128, 1, 257] if chunks == "short" else chunks
+    b = Batch(38, hq=heads, hkv=heads, dim=64, kind=kind, chunks=chunks, prefixes=[int(x) for x in rng.integers(0, 30, len(chunks))],
+              layers=1, layer=0)
+    q = b.new_rows(b.hq)
+    assert_within(prefill(b, cuda, q), *b.expect_chunks(q))
+
+
 @pytest.mark.parametrize("hq,hkv", [(4, 4), (8, 1)])
 def test_whole_prompts(cuda, hq, hkv):
     b = Batch(32, hq=hq, hkv=hkv, chunks=[300, 1, 257, 512])
