@@ -38,6 +38,7 @@ struct Prefill8Args {
     float *mid_o, *mid_lse;
     int32_t group, layer, tiles_per_split, max_splits;
     int32_t sorted, key_tiles;                // row tiles by length; about the most key tiles that one sees
+    int32_t paired;                           // a workgroup takes a chunk's i-th longest row tile and its i-th shortest
     float scale2;
 };
 
@@ -141,10 +142,11 @@ __device__ __forceinline__ bool nth_longest(const Prefill8Args& g, int per, int 
     return false;
 }
 
-// A workgroup's row tile against its range of the keys: rows row0 .. of the `rows` of chunk b, starting at batch row `start`.
+// A workgroup's row tile against its range of the keys: rows row0 .. of the `rows` of chunk b, starting at batch row `start`;
+// then, where `second` is not -1, the tile that begins there: an earlier one, with the whole keys as its range.
 template <class T, class C, int D, int WAVES, int COLS>
 __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)[Lds8<D>::kK], char (*v_lds)[Lds8<D>::kV], NaN8<D>& nans, int b,
-                                            int split, int kvh, int64_t start, int rows, int row0) {
+                                            int split, int kvh, int64_t start, int rows, int row0, int second) {
     typedef typename T::elem E;
     typedef typename T::vec8 vec8;
     typedef E vec4 __attribute__((ext_vector_type(4)));
@@ -170,40 +172,46 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
     const int nblk = (kv_len + kBlk - 1) / kBlk;
     const int num_tiles = (kv_len + 63) >> 6;
     const int tile_begin = min(split * g.tiles_per_split, num_tiles);
-    const int tile_end = split == g.max_splits - 1 ? num_tiles : min(tile_begin + g.tiles_per_split, num_tiles);
+    int tile_end = split == g.max_splits - 1 ? num_tiles : min(tile_begin + g.tiles_per_split, num_tiles);
     const int32_t* table = g.batch.block_table + (has_row ? seq * g.batch.max_blocks_per_seq : 0);
     const int num_blocks = (int)g.pool.num_blocks;
 
     // this wave's rows and Q^T: lane (row n, group c) holds dims 32 x + 8 c .. + 8 for step x
-    const int r0 = row0 + wave * 16 * COLS;
     vec8 qb[COLS][kX];
-    int last_key[COLS];                                      // a row sees keys 0 .. its own position
+    int r0, last_key[COLS], wave_last;                       // a row sees keys 0 .. its own position
+    auto take_rows = [&](int from) {
+        r0 = from + wave * 16 * COLS;
 #pragma unroll
-    for (int u = 0; u < COLS; ++u) {
-        const int r = r0 + 16 * u + n;
-        const int t = r / G;
-        const E* qrow = (const E*)g.q + (start + t) * g.q_stride + ((int64_t)kvh * G + (r - t * G)) * D;
-        last_key[u] = r < rows ? (int)min(prefix + t, room - 1) : -1;
+        for (int u = 0; u < COLS; ++u) {
+            const int r = r0 + 16 * u + n;
+            const int t = r / G;
+            const E* qrow = (const E*)g.q + (start + t) * g.q_stride + ((int64_t)kvh * G + (r - t * G)) * D;
+            last_key[u] = r < rows ? (int)min(prefix + t, room - 1) : -1;
 #pragma unroll
-        for (int x = 0; x < kX; ++x) {
-            if (r < rows) qb[u][x] = *(const vec8*)(qrow + 32 * x + 8 * c);
-            else qb[u][x] = (vec8)(E)0.f;
+            for (int x = 0; x < kX; ++x) {
+                if (r < rows) qb[u][x] = *(const vec8*)(qrow + 32 * x + 8 * c);
+                else qb[u][x] = (vec8)(E)0.f;
+            }
         }
-    }
-    const int wave_last = r0 < rows ? (int)min(prefix + (min(r0 + 16 * COLS, rows) - 1) / G, room - 1) : -1;
+        wave_last = r0 < rows ? (int)min(prefix + (min(r0 + 16 * COLS, rows) - 1) / G, room - 1) : -1;
+    };
+    take_rows(row0);
 
     // Row sums come out of the matrix cores too: a V^T row of ones makes every register of lsum the row's sum of
     // the rounded probabilities, the ones the numerator is built from.
     float4v acc[COLS][kT], lsum[COLS];
     float m_run[COLS];
     const vec8 ones = (vec8)(E)1.f;
+    auto clear = [&] {
 #pragma unroll
-    for (int u = 0; u < COLS; ++u) {
-        m_run[u] = kFar;
-        lsum[u] = (float4v){0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < COLS; ++u) {
+            m_run[u] = kFar;
+            lsum[u] = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < kT; ++t) acc[u][t] = (float4v){0.f, 0.f, 0.f, 0.f};
-    }
+            for (int t = 0; t < kT; ++t) acc[u][t] = (float4v){0.f, 0.f, 0.f, 0.f};
+        }
+    };
+    clear();
 
     const int64_t block_bytes = block_bytes8(g.pool);
     const int64_t slab = slab_offset8(g.pool, g.layer, kvh);
@@ -228,6 +236,8 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
         for (int u = 0; u < kU; ++u) ids[u] = ask_id(4 * tile + unit(u) / D);
         id_c = ask_id(4 * tile + c);
     };
+    // behind a row tile's last key tile comes the second one's first (or, of no use, the first again)
+    auto after = [&](int tile) { return tile + 1 < tile_end ? tile + 1 : tile_begin; };
     // requests the codes of `tile` and the ids of the one after it
     auto fetch = [&](int tile) {
         const int own = known_id(4 * tile + c, id_c);
@@ -243,11 +253,12 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
         }
         ex_next = scales[max(own, 0)];
         here_next = own >= 0;
-        ask_ids(tile + 1);
+        ask_ids(after(tile));
     };
-    // The tiles that every row of the workgroup sees whole end here.
-    const int full_end = max(tile_begin, min(tile_end, (int)((min(prefix + row0 / G, room - 1) + 1) >> 6)));
-    auto stage = [&](int buf, int tile) {
+    // The tiles that every row of a row tile sees whole end here.
+    auto whole_until = [&](int from, int end) { return max(tile_begin, min(end, (int)((min(prefix + from / G, room - 1) + 1) >> 6))); };
+    int full_end = whole_until(row0, tile_end);
+    auto stage = [&](int buf, bool cut) {                     // cut: some row does not see the whole tile
         unsigned found = 0;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
@@ -267,7 +278,7 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
                     keep[j] = in >= 4 ? ~0u : (1u << (8 * in)) - 1u;
                 }
             }
-            if (C::kHasNaN && tile >= full_end) {
+            if (C::kHasNaN && cut) {
                 unsigned keys = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -284,7 +295,7 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
             *(vec8*)vd = C::scaled(T{}, vreg[u][0] & keep[0], vreg[u][1] & keep[1], ev);
             *(vec8*)(vd + 64) = C::scaled(T{}, vreg[u][2] & keep[2], vreg[u][3] & keep[3], ev);
         }
-        if (C::kHasNaN && tile >= full_end) {
+        if (C::kHasNaN && cut) {
             const bool some = __ballot(found != 0) != 0;
             nans.wave[buf][wave] = some;
         }
@@ -396,47 +407,64 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
     if (tile_begin < tile_end) {
         ask_ids(tile_begin);
         fetch(tile_begin);
-        stage(0, tile_begin);
+        stage(0, tile_begin >= full_end);
         here = here_next;
         ex = ex_next;
     }
+    int buf = 0;
+    int next_full = 0;                                        // full_end of the row tile after this one
     auto iterate = [&](auto masked_tag, int from, int to) {
         for (int tile = from; tile < to; ++tile) {
-            const int buf = (tile - tile_begin) & 1;
+            const int next = after(tile);
             __syncthreads();                                  // this tile is staged; the other buffer is free
-            fetch(tile + 1);                                  // behind the last tile: one more, unused
+            fetch(next);
             if (tile * 64 <= wave_last) consume(masked_tag, buf, tile);
-            stage(buf ^ 1, tile + 1);
+            buf ^= 1;
+            stage(buf, next >= (tile + 1 < tile_end ? full_end : next_full));
             here = here_next;
             ex = ex_next;
         }
     };
-    // The tiles that every row of the workgroup sees whole, then those that hold some row's last key.  Two loops, not two
-    // bodies in one: the accumulators would be copied where the bodies meet, and the registers do not suffice for that.
-    iterate(std::false_type{}, tile_begin, full_end);
-    iterate(std::true_type{}, full_end, tile_end);
-
-    // ---- output: a lane holds, of row n of a column tile, dims 16 t + 4 c .. + 4 -------------------------------------
-#pragma unroll
-    for (int u = 0; u < COLS; ++u) {
-        const float l = lsum[u][0];
-        const int r = r0 + 16 * u + n;
-        if (r >= rows) continue;
-        const float inv = l == 0.f ? 0.f : 1.f / l;           // a row with nothing to attend to: zeros
-        const int t = r / G;
-        const int64_t head = (int64_t)kvh * G + (r - t * G);
-        if (g.max_splits == 1) {
-            E* orow = (E*)g.o + (start + t) * g.o_stride + head * D;
-#pragma unroll
-            for (int d = 0; d < kT; ++d)
-                *(vec4*)(orow + 16 * d + 4 * c) = (vec4){(E)(acc[u][d][0] * inv), (E)(acc[u][d][1] * inv),
-                                                         (E)(acc[u][d][2] * inv), (E)(acc[u][d][3] * inv)};
-        } else {
-            const int64_t at = ((start + t) * Hq + head) * g.max_splits + split;
-#pragma unroll
-            for (int d = 0; d < kT; ++d) *(float4v*)(g.mid_o + at * D + 16 * d + 4 * c) = acc[u][d] * inv;
-            if (c == 0) g.mid_lse[at] = l == 0.f ? kFar : __builtin_amdgcn_logf(l) + m_run[u];
+    const int second_end = second < 0 ? 0 : (int)((min(prefix + (second + kRows - 1) / G + 1, room) + 63) >> 6);
+    if (second >= 0) next_full = whole_until(second, second_end);
+    for (;;) {
+        // The tiles that every row of the workgroup sees whole, then those that hold some row's last key.  Two loops, not two
+        // bodies in one: the accumulators would be copied where the bodies meet, and the registers do not suffice for that.
+        iterate(std::false_type{}, tile_begin, full_end);
+        iterate(std::true_type{}, full_end, tile_end);
+        const int done = r0;
+        const bool more = second >= 0;
+        if (more) {                                               // q is on its way while the first tile's rows are written
+            take_rows(second);
+            tile_end = second_end;
+            full_end = next_full;
+            second = -1;
         }
+
+        // ---- output: a lane holds, of row n of a column tile, dims 16 t + 4 c .. + 4 -------------------------------------
+#pragma unroll
+        for (int u = 0; u < COLS; ++u) {
+            const float l = lsum[u][0];
+            const int r = done + 16 * u + n;
+            if (r >= rows) continue;
+            const float inv = l == 0.f ? 0.f : 1.f / l;           // a row with nothing to attend to: zeros
+            const int t = r / G;
+            const int64_t head = (int64_t)kvh * G + (r - t * G);
+            if (g.max_splits == 1) {
+                E* orow = (E*)g.o + (start + t) * g.o_stride + head * D;
+#pragma unroll
+                for (int d = 0; d < kT; ++d)
+                    *(vec4*)(orow + 16 * d + 4 * c) = (vec4){(E)(acc[u][d][0] * inv), (E)(acc[u][d][1] * inv),
+                                                             (E)(acc[u][d][2] * inv), (E)(acc[u][d][3] * inv)};
+            } else {
+                const int64_t at = ((start + t) * Hq + head) * g.max_splits + split;
+#pragma unroll
+                for (int d = 0; d < kT; ++d) *(float4v*)(g.mid_o + at * D + 16 * d + 4 * c) = acc[u][d] * inv;
+                if (c == 0) g.mid_lse[at] = l == 0.f ? kFar : __builtin_amdgcn_logf(l) + m_run[u];
+            }
+        }
+        if (!more) break;
+        clear();
     }
 }
 
@@ -465,14 +493,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const int len = chunk_rows(chunks_of(g.batch), b, start);
     const int rows = len * g.group;
     const int tiles = (rows + kRows - 1) / kRows;             // of this chunk
-    if (rank >= tiles) return;
-    const int row0 = (tiles - 1 - rank) * kRows;
+    if (g.paired ? 2 * rank >= tiles : rank >= tiles) return;
+    const int last = tiles - 1 - rank;
+    const int row0 = last * kRows;
+    const int second = g.paired && rank < last ? rank * kRows : -1;      // the row tile as far from the chunk's other end
     // A tile that is at most half full: one column tile a wave, on all of them, instead of two on half.  Six chunks of 1 to
     // 16 tokens of 64 q heads over 8000 to 16000 cached ones: 70 us -> 55.
-    if (COLS == 2 && rows - row0 <= kRows / 2)
-        attend_tile<T, C, D, WAVES, 1>(g, k_lds, v_lds, nans, b, split, kvh, start, rows, row0);
+    if (COLS == 2 && second < 0 && rows - row0 <= kRows / 2)
+        attend_tile<T, C, D, WAVES, 1>(g, k_lds, v_lds, nans, b, split, kvh, start, rows, row0, -1);
     else
-        attend_tile<T, C, D, WAVES, COLS>(g, k_lds, v_lds, nans, b, split, kvh, start, rows, row0);
+        attend_tile<T, C, D, WAVES, COLS>(g, k_lds, v_lds, nans, b, split, kvh, start, rows, row0, second);
 }
 
 template <class T, class C, int D>
@@ -538,13 +568,18 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     // tile shared by more rows) for long chunks that fill the chip with them -- 2048 x 4 rows over 8192 cached tokens
     // 370 us against 407 with 128, whole prompts of 8192 tokens 637 against 707, but eight of 512 tokens 46 against 42.
     const int shape = rows <= 64 ? 64 : rows > 512 && columns * mkv::cdiv(rows, 256) >= mkv::num_cus() ? 256 : 128;
-    const int64_t cells = columns * mkv::cdiv(rows, shape);
+    int64_t cells = columns * mkv::cdiv(rows, shape);
     // a launch holds fewer than 2^32 threads, the joining one up to 256 for every row
     MKV_REQUIRE(cells * 512 <= 0xffffffffll && (max_splits == 1 || rows * pool->num_kv_heads * 256 <= 0xffffffffll), "too many rows in one call");
     // Finding a workgroup's place in the order costs a few microseconds: 8 x 512 tokens 42 us, sorted 48; four ragged
     // chunks over up to 7473 cached tokens 992 us, sorted 605.
     g.key_tiles = mkv::cdiv((int64_t)tokens_per_split * max_splits, 64);
     g.sorted = batch->num_prefill_seqs > 1 && cells > 2 * mkv::num_cus() && g.key_tiles >= 32;
+    // Row tiles in pairs, a chunk's longest with its shortest, where the pairs still fill the chip: work of one size, and a
+    // start less for two tiles, since the second's first keys are fetched under the first's last.  16 x 512 tokens of 32 q and 8
+    // kv heads 72 us, single 82; 8 x 512 of 32 heads each 40.5, single 42; 8 x 256 (half the workgroups needed) 19.3 and 19.0.
+    g.paired = max_splits == 1 && !g.sorted && cells >= (shape == 256 ? 2 : 4) * mkv::num_cus();
+    if (g.paired) cells = columns * mkv::cdiv(mkv::cdiv(rows, shape), 2);
     const dim3 grid((unsigned)cells);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == MKV_F16) mkv::launch_prefill8<mkv::F16>(*pool, shape, grid, s, g);
