@@ -383,6 +383,29 @@ def test_nan_reaches_the_rows_that_see_its_key(cuda, monkeypatch, dtype, dim, hq
 
 
 @pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("dtype,kind", TYPES)
+def test_infinite_rows_stay_their_own(cuda, monkeypatch, dtype, kind, splits):
+    """A q row with an infinity or a NaN spoils its own head, not the rows that share its tile."""
+    b = Batch(39, hq=8, hkv=2, dtype=dtype, kind=kind, chunks=[40, 90], prefixes=[100, 5], dec=[200, 30])
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
+    q = b.new_rows(b.hq)
+    n = sum(b.chunks)
+    (want, bound), (want_d, bound_d) = b.expect_chunks(q[:n]), b.expect_decode(q[n:])
+    want, bound = np.concatenate([want, want_d]), np.concatenate([bound, bound_d])
+    bad = [(0, 3, np.nan), (17, 0, np.inf), (39, 7, -np.inf), (40, 1, np.nan), (129, 5, np.inf), (130, 2, np.nan), (131, 6, np.inf)]
+    for row, head, x in bad:
+        q[row, head, 11] = x
+    got = torch.cat([prefill(b, cuda, q[:n]), decode(b, cuda, q[n:]).view(-1, b.hq, b.dim)])
+    keep = np.ones((b.tokens, b.hq), dtype=bool)
+    for row, head, x in bad:
+        keep[row, head] = False
+        if np.isnan(x):
+            assert torch.isnan(got[row, head]).all()
+    at = np.nonzero(keep)
+    assert_within(got[torch.from_numpy(keep).to(cuda)], want[at], bound[at])
+
+
+@pytest.mark.parametrize("splits", [1, 3])
 def test_rows_of_no_chunk_stay(cuda, monkeypatch, splits):
     """Rows between and behind the chunks are neither read nor written."""
     monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
