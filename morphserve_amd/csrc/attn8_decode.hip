@@ -13,11 +13,11 @@
 // and, rounded, they are the second product's operand in the order in which V's sixteen bytes per head dim lie.
 // The running maximum moves only when some score has outgrown it by kLazy octaves.
 //
-// Bound: reading the codes.  64 rows of 1024 to 1536 tokens, 8 kv heads x 128: 32.4 us, 5.2 TB/s; the same loads without any
-// work 27.9 us.  128 rows and 64 q heads (int8, bf16) 61.6 us, 5.5 TB/s; 5 rows of up to 60000 tokens 96.8 us, 5.3 TB/s with
+// Bound: reading the codes.  64 rows of 1024 to 1536 tokens, 8 kv heads x 128: 31.2 us, 5.4 TB/s; the same loads without any
+// work 27.9 us.  128 rows and 64 q heads (int8, bf16) 59.7 us, 5.7 TB/s; 5 rows of up to 60000 tokens 96.2 us, 5.3 TB/s with
 // the join.  Codes of a wave's next tile are asked for as soon as their registers are free, K's between the two products and
-// V's behind the second; what remains is that a wave waits for its K with its V in flight.  A third wave per SIMD, loads in
-// pieces as single registers become free, and loads that the caches keep were no faster.
+// V's behind the second, and are waited for one by one.  A third wave per SIMD, loads in pieces as single registers become free,
+// and loads that the caches keep were no faster.
 #include <type_traits>
 
 #include "kv8.h"
@@ -98,11 +98,6 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
     const uint16_t* scales = scale_row8(g.pool, g.layer, kvh);
     const int num_blocks = (int)g.pool.num_blocks;
 
-    // table entry of block `b` of the sequence, -1 where there is none
-    auto id_of = [&](int b) {
-        const int pid = b < nblk ? table[b] : -1;
-        return pid >= 0 && pid < num_blocks ? pid : -1;
-    };
     // K: lane's row n belongs to block n / 4 of the tile; V and the scores: lane's block is c.  A block that is not
     // there is read from block 0 (inside the pool) and masked.
     auto load_k = [&](Tile8<D>& x, int pid) {
@@ -187,46 +182,59 @@ __global__ __launch_bounds__(256) void attn8_decode_kernel(const Attn8Args g) {
         after_v();
     };
 
-    // The wave's tiles are tile_begin + wave + 4 k.  Their block ids are read for sixteen tiles at a time, a lane each (lane
-    // 4 k + b: block b of tile k), one such set ahead, and handed out by lane exchange: loads complete in order, and an
-    // id read between a tile's K and V would make the next K wait for this V.
+    // The wave's tiles are tile_begin + wave + 4 k.  Loads complete in order, and where two paths meet the compiler waits for
+    // what either may have left: so a tile's block ids are asked for a tile ahead, before that tile's K, and looked at only
+    // when they are used, and nothing is loaded under a condition.
     const int first = tile_begin + wave;
     const int count = first < tile_end ? (tile_end - first + 3) >> 2 : 0;
-    auto ids_of = [&](int k0) { return id_of(4 * (first + 4 * (k0 + (lane >> 2))) + (lane & 3)); };
-    int ids = ids_of(0), ids_next = ids_of(16);
-    int pid = -1, pid_k = -1;
+    int id_k = 0, id_v = 0, pid = -1;
     unsigned ex = 0;
-    auto request_k = [&](int k) {
-        pid_k = __shfl(ids, 4 * (k & 15) + (n >> 2));
-        pid = __shfl(ids, 4 * (k & 15) + c);
-        load_k(x, pid_k);
-        ex = scales[max(pid, 0)];
+    auto ask_ids = [&](int k) {
+        const int blk = 4 * (first + 4 * k);
+        id_k = table[min(blk + (n >> 2), nblk - 1)];
+        id_v = table[min(blk + c, nblk - 1)];
     };
-    if (count > 0) {
-        request_k(0);
-        load_v(x, pid);
-    }
+    auto request_k = [&](int k) {
+        const int limit = k < count ? nblk - 4 * (first + 4 * k) : 0;      // blocks from the tile's first on
+        const int pk = n >> 2 < limit && id_k >= 0 && id_k < num_blocks ? id_k : -1;
+        pid = c < limit && id_v >= 0 && id_v < num_blocks ? id_v : -1;
+        __builtin_amdgcn_sched_barrier(0);                   // the order of the loads is the one written here
+        ask_ids(k + 1);
+        ex = scales[max(pid, 0)];
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(x, pk);
+        __builtin_amdgcn_sched_barrier(0);
+    };
     int k = 0;
     auto step = [&](auto whole_tag) {
-        const bool more = k + 1 < count;
         const bool here = pid >= 0;
-        auto after_k = [&] {
-            if (!more) return;
-            if (((k + 1) & 15) == 0) {
-                ids = ids_next;
-                ids_next = ids_of(k + 17);
-            }
-            request_k(k + 1);
-        };
-        auto after_v = [&] {
-            if (more) load_v(x, pid);
-        };
-        consume(whole_tag, first + 4 * k, here, here ? ex : 0x7f7fu, after_k, after_v);
+        consume(whole_tag, first + 4 * k, here, here ? ex : 0x7f7fu,
+                [&] {
+                    __builtin_amdgcn_sched_barrier(0);
+                    request_k(k + 1);
+                },
+                [&] {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_v(x, pid);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
     };
-    // Whole tiles, then, from the first that is not, the careful body: usually the sequence's last tile alone.  Two
-    // loops, not two bodies in one: the accumulators would be copied where the bodies meet.
-    for (; k < count && __ballot(pid < 0) == 0 && (first + 4 * k + 1) * 64 <= len; ++k) step(std::true_type{});
-    for (; k < count; ++k) step(std::false_type{});
+    if (count > 0) {
+        ask_ids(0);
+        request_k(0);
+        load_v(x, pid);
+        // q has arrived (its loads are older than the ids'), which the compiler would otherwise doubt in the loops: not
+        // knowing, it waits for all that is in flight
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < kX; ++y) asm volatile("" : "+v"(qb[y]));
+        // Whole tiles, then, from the first that is not, the careful body, which also takes the wave's last tile, behind
+        // which nothing is asked for.  Loops apart, not two bodies in one: the accumulators would be copied where the bodies meet.
+        for (; k + 1 < count && __ballot(pid < 0) == 0 && (first + 4 * k + 1) * 64 <= len; ++k) step(std::true_type{});
+        for (; k + 1 < count; ++k) step(std::false_type{});
+        const bool here = pid >= 0;
+        consume(std::false_type{}, first + 4 * k, here, here ? ex : 0x7f7fu, [] {}, [] {});
+    }
 
     // ---- the four waves' states meet in LDS --------------------------------------------------------
     const float l_all = sum_over_quarters(l_run);
