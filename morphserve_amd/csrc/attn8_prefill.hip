@@ -46,10 +46,10 @@ struct Prefill8Args {
 // consecutive ones and eight of the opposite half of the next lane group, measured with feeding products: 5.1 cycles a
 // read without conflicts and 8.0 with any.  Row distances of two 16-byte slots modulo sixteen (ten serve as well),
 // eight between blocks, with the lane group one slot further, keep every such group on sixteen different slots:
-// slot 2 n + c for K and 10 n + c for V.
+// slot 2 n + c for K (10 n + c for the shorter rows of 64 dims) and 10 n + c for V.
 template <int D>
 struct Lds8 {
-    static constexpr int kKRow = 288;
+    static constexpr int kKRow = D == 64 ? 160 : 288;
     static constexpr int kKBlock = kBlk * kKRow + 128;
     static constexpr int kK = 4 * kKBlock;
     static constexpr int kVRow = 160;            // keys 0 .. 7 of the four blocks, then keys 8 .. 15
@@ -468,8 +468,10 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
     }
 }
 
+// Two waves per SIMD at 128 head dims, by the accumulators; three at 64, of three workgroups a unit, where the softmax, as long
+// for half the products, has more to hide behind: twelve ragged prompts of 64 q heads 98 us with two, 77 with three.
 template <class T, class C, int D, int WAVES, int COLS>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn8_prefill_kernel(const Prefill8Args g) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void attn8_prefill_kernel(const Prefill8Args g) {
     constexpr int kRows = 16 * COLS * WAVES;                  // rows per workgroup
     __shared__ __attribute__((aligned(16))) char k_lds[2][Lds8<D>::kK];
     __shared__ __attribute__((aligned(16))) char v_lds[2][Lds8<D>::kV];
@@ -507,8 +509,13 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 
 template <class T, class C, int D>
 static void launch_prefill8(int shape, dim3 grid, hipStream_t s, const Prefill8Args& g) {
-    if (shape == 256) hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 8, 2>), grid, dim3(512), 0, s, g);
-    else if (shape == 128) hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 4, 2>), grid, dim3(256), 0, s, g);
+    if constexpr (D == 128) {
+        if (shape == 256) {
+            hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 8, 2>), grid, dim3(512), 0, s, g);
+            return;
+        }
+    }
+    if (shape == 128) hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 4, 2>), grid, dim3(256), 0, s, g);
     else hipLaunchKernelGGL((attn8_prefill_kernel<T, C, D, 4, 1>), grid, dim3(256), 0, s, g);
 }
 
@@ -567,7 +574,7 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     // Rows per workgroup: 64 where a chunk has no more; 256 (one workgroup of eight waves per CU, the conversions of a
     // tile shared by more rows) for long chunks that fill the chip with them -- 2048 x 4 rows over 8192 cached tokens
     // 370 us against 407 with 128, whole prompts of 8192 tokens 637 against 707, but eight of 512 tokens 46 against 42.
-    const int shape = rows <= 64 ? 64 : rows > 512 && columns * mkv::cdiv(rows, 256) >= mkv::num_cus() ? 256 : 128;
+    const int shape = rows <= 64 ? 64 : pool->head_dim == 128 && rows > 512 && columns * mkv::cdiv(rows, 256) >= mkv::num_cus() ? 256 : 128;
     int64_t cells = columns * mkv::cdiv(rows, shape);
     // a launch holds fewer than 2^32 threads, the joining one up to 256 for every row
     MKV_REQUIRE(cells * 512 <= 0xffffffffll && (max_splits == 1 || rows * pool->num_kv_heads * 256 <= 0xffffffffll), "too many rows in one call");
@@ -578,7 +585,7 @@ extern "C" int mkv_attn8_prefill(const mkv_pool8* pool, const mkv_batch* batch, 
     // Row tiles in pairs, a chunk's longest with its shortest, where the pairs still fill the chip: work of one size, and a
     // start less for two tiles, since the second's first keys are fetched under the first's last.  16 x 512 tokens of 32 q and 8
     // kv heads 72 us, single 82; 8 x 512 of 32 heads each 40.5, single 42; 8 x 256 (half the workgroups needed) 19.3 and 19.0.
-    g.paired = max_splits == 1 && !g.sorted && cells >= (shape == 256 ? 2 : 4) * mkv::num_cus();
+    g.paired = max_splits == 1 && !g.sorted && cells >= (shape == 256 ? 2 : pool->head_dim == 128 ? 4 : 6) * mkv::num_cus();
     if (g.paired) cells = columns * mkv::cdiv(mkv::cdiv(rows, shape), 2);
     const dim3 grid((unsigned)cells);
     hipStream_t s = (hipStream_t)stream;

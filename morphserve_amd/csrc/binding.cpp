@@ -311,7 +311,7 @@ Split decode_split(int64_t n, int64_t kv_heads, int64_t longest, int64_t units, 
 }
 
 // A chunk launch.  A tile of 128 rows takes 1.47 us a key tile where it has a compute unit for itself, and two that share one
-// take 1.96 (head dim 128; about two thirds of it at 64).  Over 30 random batches 1.6 % slower than the best number of
+// take 1.96; at 64 head dims 1.0, 1.4 for two and 1.9 for three.  Over 30 random batches 1.6 % slower than the best number of
 // ranges, where at least four key tiles and two workgroups per unit are 4.1 %: 1024 new tokens 30.4 us uncut and 42.9 in two
 // ranges, 128 tokens after 4096 97.5 us uncut, 35.3 in four and 25.7 in eight.
 Split prefill_split(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t keys, int64_t units, int64_t dim) {
@@ -321,7 +321,8 @@ Split prefill_split(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t row
     const int64_t have = std::max<int64_t>(seqs * kv_heads * row_tiles, 1);
     return least(keys, have, units, [&](int64_t tiles, int64_t s) {
         const double load = (double)(have * s) / (double)units;
-        const double tile = (load <= 1.0 ? 1.47 : 1.96 * std::ceil(load / 2.0)) * (0.35 + 0.65 * (double)dim / 128.0);
+        const double tile = dim > 64 ? (load <= 1.0 ? 1.47 : 1.96 * std::ceil(load / 2.0))
+                                     : (load <= 1.0 ? 1.0 : load <= 2.0 ? 1.4 : 1.9 * std::ceil(load / 3.0));
         return (double)tiles * tile + merge_time(seqs * rows * q_heads * dim, s);
     });
 }
