@@ -174,8 +174,11 @@ def attend_bound(out, mean, big, keys, most, dim, dtype):
     sum p |v|.  Scores are sums of ``dim`` exact products in 32 bits: relative to sum |q k|, off by (dim + 8) 2^-24, which is
     the absolute error of an exponent and so the relative one of a probability, above and below the fraction line: twice.
     Sums over the keys: (keys + 64) 2^-24, twice (numerator, denominator); exponentials, scales, joins of splits: 2^-18.
-    fp16 probabilities below 2^-14 lose 2^-25 each, against a sum of at least 1; outputs below 2^-14, 2^-25."""
+    fp16 probabilities below 2^-14 lose 2^-25 each, against a sum of at least 1; outputs below 2^-14, 2^-25.
+    bf16 and 32-bit numbers below 2^-126 may be taken as 0, so each of these loses less than 2^-126: a probability (against a
+    sum of at least 1, since the maximum's own is at least 1 before the division), times |v|; a probability times the scale of
+    int8 codes, times a code of at most 127; the output."""
     u = 2.0 ** -11 if dtype == "f16" else 2.0 ** -8
     rel = u + 2 * (dim + 8) * 2.0 ** -24 * big + 2 * (keys + 64) * 2.0 ** -24 + 2.0 ** -18
-    tiny = 2.0 ** -25 * (1 + keys * most) if dtype == "f16" else 2.0 ** -133
+    tiny = 2.0 ** -25 * (1 + keys * most) if dtype == "f16" else 2.0 ** -126 * (1 + keys * (most + 127))
     return u * np.abs(out) + mean * rel + tiny

@@ -322,6 +322,15 @@ def test_several_rounds_of_row_tiles(cuda, heads, chunks, kind):
     assert_within(prefill(b, cuda, q), *b.expect_chunks(q))
 
 
+@pytest.mark.parametrize("dtype,kind", [("f16", "e4m3"), ("bf16", "int8")])
+@pytest.mark.parametrize("chunks,prefixes", [([600, 513, 257], [3, 17, 0]), ([60, 700, 520], [2000, 0, 40]), ([700, 300], [0, 5])])
+def test_wide_row_tiles(cuda, dtype, kind, chunks, prefixes):
+    """Row tiles of 256, 128 head dims: in pairs, in order of length, and as they come."""
+    b = Batch(48, hq=64, hkv=64, dtype=dtype, kind=kind, chunks=chunks, prefixes=prefixes, layers=1, layer=0)
+    q = b.new_rows(b.hq)
+    assert_within(prefill(b, cuda, q), *b.expect_chunks(q))
+
+
 @pytest.mark.parametrize("hq,hkv", [(4, 4), (8, 1)])
 def test_whole_prompts(cuda, hq, hkv):
     b = Batch(32, hq=hq, hkv=hkv, chunks=[300, 1, 257, 512])
