@@ -14,15 +14,16 @@
 //
 // Bound: the matrix cores where rows are many -- 2048 tokens of 32 q heads after 8192 cached ones take 365 to 380 us, 815 to
 // 850 TFLOP/s of the two products, whole prompts of 8192 tokens 605 to 650 us (830 to 900) -- less what the softmax leaves
-// them idle: the two waves of a SIMD alternate between products and exponentials.  A wave reads its operands from LDS four ahead of the products, K's
-// last ones already V's first, and nothing is loaded under a condition, since waits where two paths meet take the worse one.
+// them idle: the two waves of a SIMD alternate between products and exponentials.  A wave reads its operands from LDS four
+// ahead of the products, during the last of K's already V's first, and nothing is loaded under a condition, since waits where
+// two paths meet take the worse one.
 #include <type_traits>
 
 #include "kv8.h"
 
 namespace mkv {
 
-static constexpr int kVAhead = 4;             // V operands requested ahead of the softmax
+static constexpr int kAhead = 4;              // operands requested from LDS ahead of their products, K's and then V's
 static constexpr float kLazyP = 8.f;
 
 // The larger of two numbers as the median of them and infinity: one instruction, where fmaxf first makes its operands
@@ -309,24 +310,23 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
         constexpr bool MASKED = decltype(masked_tag)::value;
         const char* kl = k_lds[buf] + k_rd;
         const char* vl = v_lds[buf] + v_rd;
-        // the matrix phases run at raised priority: the SIMD's other wave fills the gaps with its softmax.  K operands of
-        // the next score tile are requested ahead of the products of this one.
+        // the matrix phases run at raised priority: the SIMD's other wave fills the gaps with its softmax
         __builtin_amdgcn_s_setprio(2);
         float4v st[COLS][4];
         constexpr int kNK = 4 * kX;
-        vec8 ka[kVAhead];
+        vec8 ka[kAhead];
         auto k_operand = [&](int e) { return *(const vec8*)(kl + 4 * (e / kX) * L::kKRow + 64 * (e % kX)); };
         auto v_operand = [&](int e) { return *(const vec8*)(vl + 16 * (e >> 1) * L::kVRow + 64 * (e & 1)); };
 #pragma unroll
-        for (int e = 0; e < kVAhead; ++e) ka[e] = k_operand(e);
+        for (int e = 0; e < kAhead; ++e) ka[e] = k_operand(e);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < kNK; ++e) {
             const int j = e / kX, x = e % kX;
 #pragma unroll
             for (int u = 0; u < COLS; ++u)
-                st[u][j] = T::mfma(ka[e % kVAhead], qb[u][x], x ? st[u][j] : (float4v){0.f, 0.f, 0.f, 0.f});
-            ka[e % kVAhead] = e + kVAhead < kNK ? k_operand(e + kVAhead) : v_operand(e + kVAhead - kNK);
+                st[u][j] = T::mfma(ka[e % kAhead], qb[u][x], x ? st[u][j] : (float4v){0.f, 0.f, 0.f, 0.f});
+            ka[e % kAhead] = e + kAhead < kNK ? k_operand(e + kAhead) : v_operand(e + kAhead - kNK);
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -381,9 +381,9 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
 #pragma unroll
         for (int e = 0; e < 2 * kT; ++e) {
 #pragma unroll
-            for (int u = 0; u < COLS; ++u) acc[u][e >> 1] = T::mfma(ka[e % kVAhead], pb[u][e & 1], acc[u][e >> 1]);
-            if (e + kVAhead < 2 * kT)
-                ka[e % kVAhead] = v_operand(e + kVAhead);
+            for (int u = 0; u < COLS; ++u) acc[u][e >> 1] = T::mfma(ka[e % kAhead], pb[u][e & 1], acc[u][e >> 1]);
+            if (e + kAhead < 2 * kT)
+                ka[e % kAhead] = v_operand(e + kAhead);
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
