@@ -118,12 +118,13 @@ struct Int8 {
         }
         return (half8){h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
     }
-    // the scale in two factors, each a normal fp16 number: 2^-30, the least a block of fp16 subnormals needs, is none
+    // The scale in two factors: 2^-30, which a block of V's smallest fp16 numbers has, is no fp16 number.  A code times the
+    // first, 2^-14 at least, is exact; the second is fp16 down to its subnormals, 2^-24, and the product rounds once.
     static __device__ __forceinline__ half8 scaled(F16 t, unsigned w0, unsigned w1, unsigned e) {
         const int x = min((int)e - 127, 15);
-        const int x0 = max(x, -14), x1 = max(x - x0, -14);
+        const int x0 = max(x, -14);
         const _Float16 f0 = __builtin_bit_cast(_Float16, (unsigned short)((x0 + 15) << 10));
-        const _Float16 f1 = __builtin_bit_cast(_Float16, (unsigned short)((x1 + 15) << 10));
+        const _Float16 f1 = (_Float16)pow2_of((unsigned)(x - x0 + 127));
         return raw(t, w0, w1) * f0 * f1;
     }
     static __device__ __forceinline__ bf8 scaled(BF16, unsigned w0, unsigned w1, unsigned e) {
