@@ -54,3 +54,23 @@ def test_smallest_values(cuda, monkeypatch, dtype, kind, dim, splits):
     n = sum(b.chunks)
     assert_within(chunks(b, cuda, q[:n]), *b.expect_chunks(q[:n]), "chunks")
     assert_within(decode(b, cuda, q[n:]), *b.expect_decode(q[n:]), "decode rows")
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("dtype,kind", TYPES)
+def test_old_codes_behind_the_largest_values(cuda, monkeypatch, dtype, kind, splits):
+    """Every old code behind a sequence's last position: at the scale of the type's largest values some of them (-128, 448)
+    stand for more than the type holds, and they must not reach a row by way of a weight of 0."""
+    monkeypatch.setattr(kv8, "FORCED_SPLIT", (64, splits))
+    b = Batch(61, hq=4, hkv=2, dtype=dtype, kind=kind, chunks=[40, 67, 5], prefixes=[30, 0, 128], dec=[150, 7, 70])
+    # the largest that fp16 holds, and that 32-bit sums with weights up to 2^8 hold for bf16
+    most = 61440.0 if dtype == "f16" else 2.0 ** 118
+    set_values(b, lambda n: b.rng.choice([-1.0, 1.0, 0.5, 0.25], (n, b.dim)) * most)
+    for s, total in zip(b.seq_ids, b.total):
+        pid, last = b.table[s, (total - 1) // K.B], total % K.B
+        if last:
+            b.vc[pid, b.layer, :, :, last:] = b.rng.choice([0x80, 0x7e, 0xfe, 0x7f, 0xff], (b.hkv, b.dim, K.B - last))
+    q = b.new_rows(b.hq)
+    n = sum(b.chunks)
+    assert_within(chunks(b, cuda, q[:n]), *b.expect_chunks(q[:n]), "chunks")
+    assert_within(decode(b, cuda, q[n:]), *b.expect_decode(q[n:]), "decode rows")
