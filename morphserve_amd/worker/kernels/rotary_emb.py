@@ -117,8 +117,10 @@ def _scaled_inv_freq(rotary_dim: int, theta: float, scaling: dict, seq_len: int)
         first, last = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
         ramp = ((pair / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
         attention = scaling.get("attention_factor")
-        attention = 0.1 * math.log(factor) + 1.0 if attention is None else float(attention)
-        return inv / factor * ramp + inv * (1 - ramp), attention
+        if attention is None:                               # two scales, of the angles' and of all dims: their ratio
+            of = lambda key, usual: 0.1 * float(scaling.get(key, usual)) * math.log(factor) + 1.0  # noqa: E731
+            attention = of("mscale", 1.0) / of("mscale_all_dim", 0.0)
+        return inv / factor * ramp + inv * (1 - ramp), float(attention)
     raise ValueError(f"unknown rotary scaling {kind!r}")
 
 

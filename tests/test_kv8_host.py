@@ -106,6 +106,37 @@ def test_table_scalings():
     assert rotary_scaled_tables(d, n, theta, {**yarn, "attention_factor": 1.0}, "cpu")[0][0, 0] == 1
 
 
+def yarn_by_hand(dim, theta, factor, old, fast=32.0, slow=1.0, truncate=True):
+    """Angles of position 1, pair by pair: a pair that turns more than ``fast`` times over the trained length is kept, one that
+    turns less than ``slow`` times divided by the factor, and between them goes a ramp over the pairs' numbers."""
+    border = [dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta)) for turns in (fast, slow)]
+    lo, hi = (math.floor(border[0]), math.ceil(border[1])) if truncate else border
+    lo, hi = max(lo, 0), min(hi, dim - 1)
+    angles = []
+    for i in range(dim // 2):
+        plain, part = theta ** (-2 * i / dim), min(max((i - lo) / (hi - lo), 0), 1)
+        angles.append(plain * (1 - part) + plain / factor * part)
+    return np.asarray(angles)
+
+
+def angles_of(tables):
+    return np.arctan2(tables[1].double().numpy(), tables[0].double().numpy())[1]
+
+
+@pytest.mark.parametrize("scales,want", [
+    (dict(mscale=1.0, mscale_all_dim=1.0), 1.0), (dict(mscale=0.707, mscale_all_dim=0.707), 1.0),
+    (dict(mscale=1.0), 0.1 * math.log(40) + 1), (dict(mscale_all_dim=0), 0.1 * math.log(40) + 1),
+    (dict(mscale=0.5, mscale_all_dim=2.0), (0.05 * math.log(40) + 1) / (0.2 * math.log(40) + 1)),
+    (dict(mscale=0.5, mscale_all_dim=2.0, attention_factor=1.25), 1.25)])
+def test_yarn_with_two_scales(scales, want):
+    """64 rotary dims, 4096 trained positions, a factor of 40: the cosines' and sines' factor is the ratio of the two scales."""
+    config = {"rope_type": "yarn", "factor": 40, "original_max_position_embeddings": 4096, "beta_fast": 32, "beta_slow": 1, **scales}
+    tables = rotary_scaled_tables(64, 8, 10000.0, config, "cpu")
+    size = torch.hypot(tables[0].double(), tables[1].double())
+    assert np.allclose(size.numpy(), want, rtol=2.0 ** -22)
+    assert np.allclose(angles_of(tables), yarn_by_hand(64, 10000.0, 40, 4096), rtol=2.0 ** -22, atol=0)
+
+
 @pytest.mark.parametrize("args", [(7, 4), (0, 4), (8, 4, 1e4, {"rope_type": "linear", "factor": 0.5}), (8, 4, 1e4, {"rope_type": "odd", "factor": 2, "original_max_position_embeddings": 8}),
                                   (8, 4, 1e4, {"rope_type": "yarn", "factor": 2}), (2, 4, 1e4, {"rope_type": "dynamic", "factor": 2, "original_max_position_embeddings": 8}),
                                   (8, 4, 1e4, {"rope_type": "llama3", "factor": 2, "low_freq_factor": 4, "high_freq_factor": 4, "original_max_position_embeddings": 8})])
