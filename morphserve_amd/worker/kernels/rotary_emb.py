@@ -114,7 +114,10 @@ def _scaled_inv_freq(rotary_dim: int, theta: float, scaling: dict, seq_len: int)
     if kind == "yarn":                                      # the ramp runs over the pairs' numbers
         fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
         pair_of = lambda turns: rotary_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
-        first, last = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
+        first, last = pair_of(fast), pair_of(slow)
+        if scaling.get("truncate", True):                   # the ramp's ends at whole pairs
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rotary_dim - 1)
         ramp = ((pair / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
         attention = scaling.get("attention_factor")
         if attention is None:                               # two scales, of the angles' and of all dims: their ratio

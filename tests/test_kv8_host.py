@@ -137,6 +137,17 @@ def test_yarn_with_two_scales(scales, want):
     assert np.allclose(angles_of(tables), yarn_by_hand(64, 10000.0, 40, 4096), rtol=2.0 ** -22, atol=0)
 
 
+@pytest.mark.parametrize("truncate", [True, False, None])
+@pytest.mark.parametrize("dim,theta,factor,old", [(64, 150000.0, 32, 4096), (128, 1e6, 4, 32768), (32, 10000.0, 8, 1024)])
+def test_yarn_ramp_with_and_without_whole_ends(dim, theta, factor, old, truncate):
+    config = {"rope_type": "yarn", "factor": factor, "original_max_position_embeddings": old}
+    if truncate is not None:
+        config["truncate"] = truncate
+    got = angles_of(rotary_scaled_tables(dim, 8, theta, config, "cpu"))
+    want, other = (yarn_by_hand(dim, theta, factor, old, truncate=t) for t in (truncate is not False, truncate is False))
+    assert np.allclose(got, want, rtol=2.0 ** -22, atol=0) and not np.allclose(got, other, rtol=1e-3, atol=0)
+
+
 @pytest.mark.parametrize("args", [(7, 4), (0, 4), (8, 4, 1e4, {"rope_type": "linear", "factor": 0.5}), (8, 4, 1e4, {"rope_type": "odd", "factor": 2, "original_max_position_embeddings": 8}),
                                   (8, 4, 1e4, {"rope_type": "yarn", "factor": 2}), (2, 4, 1e4, {"rope_type": "dynamic", "factor": 2, "original_max_position_embeddings": 8}),
                                   (8, 4, 1e4, {"rope_type": "llama3", "factor": 2, "low_freq_factor": 4, "high_freq_factor": 4, "original_max_position_embeddings": 8})])
