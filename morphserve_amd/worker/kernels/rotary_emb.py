@@ -84,47 +84,90 @@ def rotary_embedding_and_store_kvcache(
         cur_layer, 1, _capi.current_stream()))
 
 
+# the keys that each scaling rule reads, and those that any dict may hold: the rule's name, and what the arguments say already
+_SCALING_KEYS = {
+    "default": (),
+    "linear": ("factor",),
+    "dynamic": ("factor",),
+    "llama3": ("factor", "low_freq_factor", "high_freq_factor"),
+    "yarn": ("factor", "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"),
+}
+_COMMON_KEYS = ("rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings", "finetuned")
+
+
+def _scaling_rule(scaling: dict, theta: float) -> str:
+    """The rule's name; ``ValueError`` for one that is not known, and for keys that it would leave unread."""
+    kinds = {str(scaling[key]) for key in ("rope_type", "type") if scaling.get(key) is not None} or {"default"}
+    if len(kinds) > 1 or not kinds <= _SCALING_KEYS.keys():
+        raise ValueError(f"unknown rotary scaling {' / '.join(sorted(map(repr, kinds)))}")
+    kind = kinds.pop()
+    unread = [key for key in scaling if key not in _SCALING_KEYS[kind] + _COMMON_KEYS]
+    if unread:
+        raise ValueError(f"rotary scaling {kind!r} does not know {', '.join(map(repr, unread))}")
+    if _number(scaling, "rope_theta", theta) != theta:
+        raise ValueError(f"rope_theta is {theta}, the scaling's {scaling['rope_theta']}")
+    return kind
+
+
+def _number(scaling: dict, key: str, usual: Optional[float] = None) -> float:
+    value = scaling.get(key)
+    if value is None:
+        value = usual
+    try:
+        value = float(value)
+    except (TypeError, ValueError):
+        raise ValueError(f"rotary scaling needs a number as {key!r}, got {value!r}") from None
+    if not math.isfinite(value):
+        raise ValueError(f"rotary scaling needs a finite {key!r}, got {value}")
+    return value
+
+
 def _scaled_inv_freq(rotary_dim: int, theta: float, scaling: dict, seq_len: int) -> Tuple[torch.Tensor, float]:
     """Inverse frequencies in 64 bits and the factor of the cosines and sines, for one scaling rule."""
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    kind = _scaling_rule(scaling, theta)
     pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     inv = theta ** (-pair / rotary_dim)
     if kind == "default":
         return inv, 1.0
-    factor = float(scaling["factor"])
+    factor = _number(scaling, "factor")
     if factor < 1:
         raise ValueError(f"a rotary scaling factor is at least 1, got {factor}")
     if kind == "linear":                                    # positions / factor
         return inv / factor, 1.0
-    old = float(scaling.get("original_max_position_embeddings", 0))
+    old = _number(scaling, "original_max_position_embeddings")
     if old <= 0:
-        raise ValueError(f"rotary scaling {kind!r} needs original_max_position_embeddings")
+        raise ValueError(f"original_max_position_embeddings must be positive, got {old}")
     if kind == "dynamic":                                   # a larger base, by how far the context exceeds the trained one
         if rotary_dim <= 2:
             raise ValueError("rotary scaling 'dynamic' needs a rotary dim above 2")
         grown = max(1.0, factor * max(seq_len, old) / old - (factor - 1))
         return (theta * grown ** (rotary_dim / (rotary_dim - 2))) ** (-pair / rotary_dim), 1.0
     if kind == "llama3":                                    # slow pairs / factor, fast pairs kept, a ramp between
-        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        low, high = _number(scaling, "low_freq_factor", 1.0), _number(scaling, "high_freq_factor", 4.0)
         if high <= low:
             raise ValueError("high_freq_factor must exceed low_freq_factor")
         turns = old * inv / (2 * math.pi)
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         return inv * keep + inv / factor * (1 - keep), 1.0
-    if kind == "yarn":                                      # the ramp runs over the pairs' numbers
-        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
-        pair_of = lambda turns: rotary_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
-        first, last = pair_of(fast), pair_of(slow)
-        if scaling.get("truncate", True):                   # the ramp's ends at whole pairs
-            first, last = math.floor(first), math.ceil(last)
-        first, last = max(first, 0), min(last, rotary_dim - 1)
-        ramp = ((pair / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
-        attention = scaling.get("attention_factor")
-        if attention is None:                               # two scales, of the angles' and of all dims: their ratio
-            of = lambda key, usual: 0.1 * float(scaling.get(key, usual)) * math.log(factor) + 1.0  # noqa: E731
-            attention = of("mscale", 1.0) / of("mscale_all_dim", 0.0)
-        return inv / factor * ramp + inv * (1 - ramp), float(attention)
-    raise ValueError(f"unknown rotary scaling {kind!r}")
+    # yarn: the ramp runs over the pairs' numbers
+    fast, slow = _number(scaling, "beta_fast", 32.0), _number(scaling, "beta_slow", 1.0)
+    if not fast > slow > 0 or theta <= 1:
+        raise ValueError(f"rotary scaling 'yarn' needs beta_fast > beta_slow > 0 and a base above 1, got {fast}, {slow}, {theta}")
+    pair_of = lambda turns: rotary_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+    first, last = pair_of(fast), pair_of(slow)
+    truncate = scaling.get("truncate")
+    if truncate not in (None, True, False):
+        raise ValueError(f"truncate is true or false, got {truncate!r}")
+    if truncate is None or truncate:                        # the ramp's ends at whole pairs
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rotary_dim - 1)
+    ramp = ((pair / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
+    if scaling.get("attention_factor") is not None:
+        attention = _number(scaling, "attention_factor")
+    else:                                                   # two scales, of the angles' and of all dims: their ratio
+        of = lambda key, usual: 0.1 * _number(scaling, key, usual) * math.log(factor) + 1.0  # noqa: E731
+        attention = of("mscale", 1.0) / of("mscale_all_dim", 0.0)
+    return inv / factor * ramp + inv * (1 - ramp), attention
 
 
 def rotary_scaled_tables(rotary_dim: int, num_positions: int, rope_theta: float = 10000.0,
@@ -132,14 +175,19 @@ def rotary_scaled_tables(rotary_dim: int, num_positions: int, rope_theta: float 
                          device: str = "cuda") -> Tuple[torch.Tensor, torch.Tensor]:
     """fp32 ``(cos, sin)`` [num_positions, rotary_dim / 2], angles computed in 64 bits (a far position times a frequency
     loses its phase in 32).  ``rope_scaling``: ``None``, a number (linear), or the dict of a model's config with
-    ``rope_type`` one of ``default``, ``linear``, ``dynamic``, ``llama3``, ``yarn``."""
+    ``rope_type`` one of ``default``, ``linear``, ``dynamic``, ``llama3``, ``yarn`` (``mscale``, ``mscale_all_dim`` and
+    ``truncate`` included).  ``dynamic`` takes ``num_positions`` as the context's length.  A rule, or a key of the dict, that is
+    not known is refused with ``ValueError``, and so is a ``rope_theta`` in it that differs from the argument."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
     if rope_scaling is None:
         rope_scaling = {}
     elif not isinstance(rope_scaling, dict):
-        rope_scaling = {"rope_type": "linear", "factor": float(rope_scaling)}
-    inv, mul = _scaled_inv_freq(rotary_dim, float(rope_theta), rope_scaling, num_positions)
+        rope_scaling = {"rope_type": "linear", "factor": rope_scaling}
+    theta = float(rope_theta)
+    if not (theta > 0 and math.isfinite(theta)) or num_positions < 0:
+        raise ValueError(f"rotary tables need a positive base and a number of positions, got {rope_theta}, {num_positions}")
+    inv, mul = _scaled_inv_freq(rotary_dim, theta, rope_scaling, num_positions)
     angle = torch.outer(torch.arange(num_positions, dtype=torch.float64, device=device), inv.to(device))
     return (torch.cos(angle) * mul).float(), (torch.sin(angle) * mul).float()
 

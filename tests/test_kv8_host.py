@@ -156,6 +156,44 @@ def test_table_refusals(args):
         rotary_scaled_tables(*args, device="cpu")
 
 
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "longrope"}, {"type": "su", "factor": 4}, {"rope_type": "default", "type": "linear", "factor": 2},
+    {"rope_type": "linear"}, {"rope_type": "linear", "factor": None}, {"rope_type": "linear", "factor": "two"},
+    {"rope_type": "linear", "factor": math.nan}, {"rope_type": "linear", "factor": math.inf}, math.nan, "two",
+    {"rope_type": "dynamic", "factor": 2}, {"rope_type": "llama3", "factor": 2, "original_max_position_embeddings": None},
+    {"rope_type": "yarn", "original_max_position_embeddings": 64},
+    {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": -64},
+    {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 64, "beta_fast": 1, "beta_slow": 32},
+    {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 64, "beta_slow": 0},
+    {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 64, "truncate": "no"},
+    {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 64, "attention_factor": "big"},
+    {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 64, "low_freq_factor": 1},
+    {"rope_type": "linear", "factor": 2, "mscale": 1.0}, {"rope_type": "default", "factor": 2},
+    {"rope_type": "default", "mrope_section": [16, 24, 24]}, {"nonsense": 3}, {"rope_type": "linear", "factor": 2, "rope_theta": 5e5},
+    {"rope_type": ["linear"], "factor": 2}])
+def test_scalings_that_are_refused(scaling):
+    """Rules and keys that are not known, and values that are no numbers: a table made without them would be a wrong one."""
+    with pytest.raises(ValueError):
+        rotary_scaled_tables(32, 4, 1e4, scaling, "cpu")
+
+
+@pytest.mark.parametrize("args", [(32, -1), (32, 4, 0.0), (32, 4, math.nan), (32, 4, 1.0, {"type": "yarn", "factor": 2, "original_max_position_embeddings": 64})])
+def test_bases_and_lengths_that_are_refused(args):
+    with pytest.raises(ValueError):
+        rotary_scaled_tables(*args, device="cpu")
+
+
+def test_keys_that_say_nothing_of_the_angles():
+    plain = rotary_scaled_tables(32, 40, 5e5, {"type": "linear", "factor": 2}, "cpu")
+    same = {"rope_type": "linear", "type": "linear", "factor": 2.0, "rope_theta": 5e5, "original_max_position_embeddings": 64,
+            "finetuned": True, "partial_rotary_factor": 0.5}
+    assert all(torch.equal(x, y) for x, y in zip(plain, rotary_scaled_tables(32, 40, 5e5, same, "cpu")))
+    yarn = {"type": "yarn", "factor": 4, "original_max_position_embeddings": 64}
+    none = dict.fromkeys(("rope_type", "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"))
+    for x, y in zip(rotary_scaled_tables(32, 40, 5e5, yarn, "cpu"), rotary_scaled_tables(32, 40, 5e5, {**yarn, **none}, "cpu")):
+        assert torch.equal(x, y)
+
+
 # ---- the cache object -----------------------------------------------------------------------------------------------------
 def test_cache_object():
     cache = allocate_kv8_cache(5, (2, 3, 16, 64), torch.int8, "cpu")
