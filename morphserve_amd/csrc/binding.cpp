@@ -121,6 +121,17 @@ int64_t out_rows_of(const at::Tensor& o, const char* what, const at::Tensor& lik
     return stride;
 }
 
+// The state's softmax scale.
+double scale_of(PyObject* st) {
+    const Attr scale(st, names.softmax_scale);
+    const double x = PyFloat_AsDouble(scale.value);
+    if (x == -1.0 && PyErr_Occurred()) {
+        PyErr_Clear();
+        refuse("softmax_scale must be a number");
+    }
+    return x;
+}
+
 const int32_t* ints_of(const at::Tensor& t, const char* what, const at::Tensor& like, int64_t least) {
     if (t.scalar_type() != at::kInt || t.device() != like.device() || t.numel() < least || !t.is_contiguous())
         refuse("%s must hold %lld contiguous int32 on the rows' device", what, (long long)least);
@@ -435,9 +446,7 @@ int decode(PyObject* const* a, Py_ssize_t count) {
     const int64_t qs = rows_of(q, "q", q, n, heads, p.head_dim), os = out_rows_of(o, "o", q, n, heads, p.head_dim);
     const int32_t layer = small(a[9], "cur_layer");
     if (n == 0) return MKV_OK;
-    const Attr scale(a[8], names.softmax_scale);
-    const double softmax_scale = PyFloat_AsDouble(scale.value);
-    if (softmax_scale == -1.0 && PyErr_Occurred()) throw Refused{};
+    const double softmax_scale = scale_of(a[8]);
     const int64_t room = b.max_blocks_per_seq * kBlock, known = int_attr(a[8], names.max_decoding_len);
     const OnDevice on(q);
     const Split s = a[11] != Py_None ? forced_split(a[11])
@@ -463,9 +472,7 @@ int prefill(PyObject* const* a, Py_ssize_t count) {
     const int64_t max_prefix = integer(a[12], "max_prefix_len");
     if (max_prefix < 0) refuse("max_prefix_len is negative");
     if (b.num_prefill_seqs == 0 || tokens == 0) return MKV_OK;
-    const Attr scale(a[8], names.softmax_scale);
-    const double softmax_scale = PyFloat_AsDouble(scale.value);
-    if (softmax_scale == -1.0 && PyErr_Occurred()) throw Refused{};
+    const double softmax_scale = scale_of(a[8]);
     const int64_t room = b.max_blocks_per_seq * kBlock;
     const int64_t keys = !b.prefix_lens ? b.max_prefill_len : max_prefix > 0 ? b.max_prefill_len + max_prefix : room;
     const OnDevice on(q);
@@ -475,6 +482,26 @@ int prefill(PyObject* const* a, Py_ssize_t count) {
     const Scratch scratch(q, (int64_t)tokens * heads, s.count, p.head_dim);
     return entry<decltype(mkv_attn8_prefill)>(a[0])(&p, &b, dtype, q.const_data_ptr(), o.data_ptr(), qs, os, heads, (float)softmax_scale,
                                                     layer, s.tokens, s.count, scratch.mid_o, scratch.mid_lse, stream_of(q));
+}
+
+// (q, o, model, state, max_prefix_len): refuses what the attention of a step would, before its append is launched.
+int section(PyObject* const* a, Py_ssize_t count) {
+    expect(count, 5);
+    const at::Tensor &q = tensor(a[0], "q"), &o = tensor(a[1], "o");
+    dtype_of(q, "q");
+    const int64_t prefill = int_attr(a[3], names.num_prefill_tokens), decode = int_attr(a[3], names.num_decoding_seqs);
+    if (prefill < 0 || decode < 0) refuse("num_prefill_tokens or num_decoding_seqs is negative");
+    if (decode > 65535) refuse("at most 65535 decode rows per call");
+    const int64_t heads = int_attr(a[2], names.num_q_heads), kv_heads = int_attr(a[2], names.num_kv_heads), dim = int_attr(a[2], names.head_dim);
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 16)
+        refuse("num_q_heads %lld must be 1 to 16 times num_kv_heads %lld", (long long)heads, (long long)kv_heads);
+    const int64_t qs = rows_of(q, "q", q, prefill + decode, heads, dim), os = out_rows_of(o, "o", q, prefill + decode, heads, dim);
+    if ((((uintptr_t)q.const_data_ptr()) & 15) || (qs & 7)) refuse("q rows must be 16-byte aligned");
+    if (integer(a[4], "max_prefix_len") < 0) refuse("max_prefix_len is negative");
+    const double scale = scale_of(a[3]);
+    if (prefill && !(scale > 0)) refuse("softmax_scale must be positive");
+    if (prefill && ((((uintptr_t)o.const_data_ptr()) & 15) || (os & 7))) refuse("o rows must be 16-byte aligned");
+    return MKV_OK;
 }
 
 // No C++ exception leaves a function of the module.
@@ -539,6 +566,7 @@ PyMethodDef methods[] = {
     {"store", (PyCFunction)(void (*)(void))call<store>, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction)(void (*)(void))call<decode>, METH_FASTCALL, nullptr},
     {"prefill", (PyCFunction)(void (*)(void))call<prefill>, METH_FASTCALL, nullptr},
+    {"section", (PyCFunction)(void (*)(void))call<section>, METH_FASTCALL, nullptr},
     {"pool_fields", (PyCFunction)(void (*)(void))pool_fields, METH_FASTCALL, nullptr},
     {"decode_split", (PyCFunction)(void (*)(void))py_decode_split, METH_FASTCALL, nullptr},
     {"prefill_split", (PyCFunction)(void (*)(void))py_prefill_split, METH_FASTCALL, nullptr},

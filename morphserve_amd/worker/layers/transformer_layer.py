@@ -28,6 +28,7 @@ from typing import List, Optional, Tuple, Union
 
 import torch
 
+from ... import _capi
 from ...kv8_cache import KV8Cache
 from ..kernels.kv8 import (chunked_prefill_attention_8bit, paged_attention_8bit, rotary_embedding_and_store_kvcache_8bit,
                            store_kvcache_8bit)
@@ -122,6 +123,8 @@ def _attention_section_8bit(q, k, v, o, cache, v_cache, k_cache_new, v_cache_new
         raise ValueError("an 8-bit cache is one object: no v_cache and no extension segments beside it")
     if bool(getattr(st, "ignore_kvcache", False)) or keep_rotated_inputs or decoding_piggyback_stream is not None:
         raise ValueError("ignore_kvcache, keep_rotated_inputs and a second stream are not supported over the 8-bit cache")
+    # what the attention would refuse is refused here: behind the append q would be rotated and the cache grown already
+    _capi.binding().section(q, o, model_config, st, max_prefix_len)
     if rotary:
         if rotary_tables is None:
             raise ValueError("rotary over the 8-bit cache needs rotary_tables")

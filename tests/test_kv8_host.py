@@ -316,3 +316,50 @@ def test_rows_on_the_cpu_are_refused():
     cos, sin = rotary_scaled_tables(32, 4, device="cpu")
     with pytest.raises(ValueError):
         rotary_embedding(torch.zeros(2, 2, 64, dtype=torch.float16), None, torch.zeros(2, dtype=torch.int32), cos, sin)
+
+
+# ---- the attention section ------------------------------------------------------------------------------------------------
+def section(monkeypatch, **change):
+    """``attention_section`` over an 8-bit cache on the CPU, its launches recorded instead of made: what was launched."""
+    from helpers import Cfg
+    from morphserve_amd.worker.layers import transformer_layer as layer
+    calls = []
+    for name in ("store_kvcache_8bit", "rotary_embedding_and_store_kvcache_8bit", "chunked_prefill_attention_8bit", "paged_attention_8bit"):
+        monkeypatch.setattr(layer, name, lambda *a, _name=name, **kw: calls.append(_name))
+    cache = allocate_kv8_cache(4, (1, 2, 16, 64), device="cpu")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    a = dict(q=torch.zeros(6, 4, 64, dtype=torch.float16), o=torch.zeros(6, 256, dtype=torch.float16), heads=4, softmax_scale=0.125,
+             max_prefix_len=0, prefill=5, dec=1)
+    a.update(change)
+    k = torch.zeros(6, 2, 64, dtype=torch.float16)
+    st = Cfg(seq_ids=i32(0, 1), num_prefill_seqs=1, num_prefill_tokens=a["prefill"], prefill_seq_start_locs=i32(0), prefill_seq_lens=i32(5),
+             max_prefill_len=5, num_decoding_seqs=a["dec"], decoding_seq_lens=i32(3), max_decoding_len=3, softmax_scale=a["softmax_scale"])
+    model = Cfg(num_layers=1, num_q_heads=a["heads"], num_kv_heads=2, head_dim=64)
+    tables = rotary_scaled_tables(64, 8, device="cpu")
+    try:
+        layer.attention_section(a["q"], k, k, a["o"], cache, None, [], [], torch.zeros(2, 2, dtype=torch.int32), model,
+                                Cfg(block_size=16, max_blocks_per_seq=2), st, 0, rotary_tables=tables, max_prefix_len=a["max_prefix_len"])
+    except ValueError:
+        return "refused" if not calls else calls
+    return calls
+
+
+def test_section_launches(monkeypatch):
+    want = ["rotary_embedding_and_store_kvcache_8bit", "chunked_prefill_attention_8bit", "paged_attention_8bit"]
+    assert section(monkeypatch) == want
+    assert section(monkeypatch, o=torch.zeros(6, 4, 64, dtype=torch.float16)) == want
+    assert section(monkeypatch, q=torch.zeros(6, 8, 64, dtype=torch.float16)[:, 2:6], o=torch.zeros(6, 300, dtype=torch.float16)[:, 8:264][:, :256]) == "refused"
+    assert section(monkeypatch, o=torch.zeros(6, 304, dtype=torch.float16)[:, 8:264]) == want
+
+
+@pytest.mark.parametrize("change", [
+    dict(o=torch.zeros(5, 256, dtype=torch.float16)), dict(o=torch.zeros(6, 255, dtype=torch.float16)), dict(o=torch.zeros(6, 256)),
+    dict(o=torch.zeros(6, 512, dtype=torch.float16)[:, ::2]), dict(o=torch.zeros(1, 256, dtype=torch.float16).expand(6, 256)),
+    dict(o=torch.zeros(6 * 256 + 1, dtype=torch.float16)[1:].view(6, 256)), dict(o=None), dict(q=torch.zeros(6, 3, 64, dtype=torch.float16)),
+    dict(q=torch.zeros(7, 4, 64, dtype=torch.float16)), dict(softmax_scale=0.0), dict(softmax_scale=-1.0), dict(softmax_scale=math.nan),
+    dict(softmax_scale="big"), dict(max_prefix_len=-1), dict(max_prefix_len=0.5), dict(prefill=6), dict(dec=2), dict(dec=-1, prefill=7),
+    dict(heads=3, q=torch.zeros(6, 3, 64, dtype=torch.float16), o=torch.zeros(6, 192, dtype=torch.float16)),
+    dict(heads=34, q=torch.zeros(6, 34, 64, dtype=torch.float16), o=torch.zeros(6, 34 * 64, dtype=torch.float16))])
+def test_section_refuses_before_it_launches(monkeypatch, change):
+    """A call that its attention would refuse leaves q and the cache as they are: done again, it must not rotate q twice."""
+    assert section(monkeypatch, **change) == "refused"
