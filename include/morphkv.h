@@ -498,7 +498,7 @@ int mkv_store8(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, con
  * tokens_per_split (a multiple of 64) and max_splits as there; mid_o (fp32
  * [n, Hq, max_splits, D], 16-byte aligned) and mid_lse (fp32 [n, Hq, max_splits])
  * may be NULL when max_splits is 1.  At most 65535 rows; tokens_per_split times
- * max_splits at most 2^33.  Sums are held in 32 bits with weights up to 2^8: values
+ * max_splits at most 2^33, max_splits below 2^24.  Sums are held in 32 bits with weights up to 2^8: values
  * of V beyond 2^119 (bf16) may overflow them. */
 int mkv_attn8_decode(const mkv_pool8* pool, const mkv_batch* batch, int32_t dtype, const void* q,
                      void* o, int64_t q_stride, int64_t o_stride, int32_t num_q_heads,

@@ -428,6 +428,7 @@ extern "C" int mkv_attn8_decode(const mkv_pool8* pool, const mkv_batch* batch, i
     MKV_REQUIRE(max_splits >= 1, "max_splits must be >= 1");
     // tile and block numbers, those behind the last key included, are 32-bit
     MKV_REQUIRE((int64_t)tokens_per_split * max_splits <= (int64_t)1 << 33, "%d ranges of %d tokens are too long", max_splits, tokens_per_split);
+    MKV_REQUIRE((int64_t)max_splits * 256 <= 0xffffffffll, "%d ranges are too many", max_splits);        // threads of the launch
     MKV_REQUIRE(max_splits == 1 || (mid_o && mid_lse), "scratch buffers are NULL");
     MKV_REQUIRE(((uintptr_t)mid_o & 15) == 0 && ((uintptr_t)mid_lse & 3) == 0, "mid_o must be 16-byte aligned, mid_lse 4-byte aligned");
     MKV_REQUIRE(((uintptr_t)q & 15) == 0 && (q_stride & 7) == 0, "q rows must be 16-byte aligned");

@@ -363,3 +363,10 @@ def test_section_launches(monkeypatch):
 def test_section_refuses_before_it_launches(monkeypatch, change):
     """A call that its attention would refuse leaves q and the cache as they are: done again, it must not rotate q twice."""
     assert section(monkeypatch, **change) == "refused"
+
+
+@pytest.mark.parametrize("entry", ["mkv_attn8_decode", "mkv_attn8_prefill"])
+def test_more_ranges_than_a_launch_has_threads(entry):
+    """2^24 ranges of 256 threads each are 2^32 threads."""
+    for splits in (2 ** 24, 2 ** 25, 2 ** 27):
+        assert attn(entry, tps=64, splits=splits) == _capi.MKV_EINVAL, splits
