@@ -115,10 +115,10 @@ def build_library(verbose: bool = True, jobs: int = 8, diag: bool = True) -> str
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         binding = ex.submit(_build_binding)
         objs = list(ex.map(lambda w: (w[1], _compile(*w)), work))
-        binding.result()
     _link([o for d, o in objs if d == obj_dir], LIB_PATH)
     if diag:
         _link([o for d, o in objs if d == diag_dir], DIAG_LIB_PATH)
+    binding.result()                        # the libraries need neither Python nor torch: they are there if this fails
     if verbose:
         for path in (LIB_PATH, DIAG_LIB_PATH, BINDING_PATH) if diag else (LIB_PATH, BINDING_PATH):
             print(f"built {path} ({os.path.getsize(path) / 1024:.0f} KiB)")

@@ -370,3 +370,21 @@ def test_more_ranges_than_a_launch_has_threads(entry):
     """2^24 ranges of 256 threads each are 2^32 threads."""
     for splits in (2 ** 24, 2 ** 25, 2 ** 27):
         assert attn(entry, tps=64, splits=splits) == _capi.MKV_EINVAL, splits
+
+
+# ---- the native module beside the library -----------------------------------------------------------------------------------
+def test_library_is_linked_without_the_native_module(monkeypatch, tmp_path):
+    """A tree whose Python or torch headers do not fit the module still yields the library, which needs neither."""
+    from morphserve_amd.csrc import build
+    linked = []
+
+    def no_module():
+        raise RuntimeError("no Python.h")
+
+    monkeypatch.setattr(build, "HERE", str(tmp_path))
+    monkeypatch.setattr(build, "_compile", lambda src, obj_dir, defines=(): src)
+    monkeypatch.setattr(build, "_link", lambda objs, out: linked.append(out))
+    monkeypatch.setattr(build, "_build_binding", no_module)
+    with pytest.raises(RuntimeError, match="Python.h"):
+        build.build_library(verbose=False)
+    assert linked == [build.LIB_PATH, build.DIAG_LIB_PATH]
