@@ -240,13 +240,18 @@ def binding():
     if _binding is None:
         import importlib.machinery
         import importlib.util
+        import sysconfig
         import torch  # noqa: F401  (its libraries are the module's)
-        path = os.path.join(_HERE, "csrc", "_binding.so")
+        path = os.path.join(_HERE, "csrc", "_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
         if not os.path.exists(path):
             raise ImportError(f"{path} is missing: build it with `python -m morphserve_amd.csrc.build`")
         loader = importlib.machinery.ExtensionFileLoader("_binding", path)
-        _binding = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
-        loader.exec_module(_binding)
+        try:
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+            loader.exec_module(module)
+        except ImportError as e:            # of another torch, say
+            raise ImportError(f"{path} does not load: build it again with `python -m morphserve_amd.csrc.build` ({e})") from e
+        _binding = module
     return _binding
 
 

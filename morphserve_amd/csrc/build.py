@@ -6,8 +6,9 @@ plus ``diag.hip``: the same entry points and, on top, the switches and measureme
 ``include/morphkv_diag.h`` (kernel variants, per-launch event timing, per-workgroup time stamps,
 calibration loops).  Benchmarks and tests that need those load the twin; the package never does.
 
-``_binding.so`` is the host side of the 8-bit cache's and the rotary operators (argument checks and the call, a CPython
-module over torch's C++ tensors); it holds no kernel and takes the library's entries by address.
+``_binding`` (with the interpreter's tag in its file name) is the host side of the 8-bit cache's and the rotary
+operators: argument checks and the call, a CPython module over torch's C++ tensors; it holds no kernel and takes the
+library's entries by address.
 
 Usage: ``python -m morphserve_amd.csrc.build`` or ``build_library()``.
 The shared objects land next to the sources so that they travel with the tree.
@@ -18,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -26,7 +28,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "libmorphkv.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 DIAG_LIB_PATH = os.path.join(HERE, "libmorphkv_diag.so")
-BINDING_PATH = os.path.join(HERE, "_binding.so")
+BINDING_PATH = os.path.join(HERE, "_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 SOURCES = [
     "core.hip",
@@ -74,7 +76,6 @@ def _compile(src: str, obj_dir: str, defines=()) -> str:
 
 
 def _build_binding() -> None:
-    import sysconfig
     from torch.utils.cpp_extension import include_paths
     import torch
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -103,7 +104,7 @@ def _link(objs, out: str) -> None:
 
 def build_library(verbose: bool = True, jobs: int = 8, diag: bool = True) -> str:
     """Compile every source and link ``libmorphkv.so`` (and, with ``diag``, its diagnostic twin)
-    and ``_binding.so``; always rebuilds."""
+    and the ``_binding`` module; always rebuilds."""
     obj_dir = os.path.join(HERE, "build")
     diag_dir = os.path.join(obj_dir, "diag")
     os.makedirs(diag_dir if diag else obj_dir, exist_ok=True)

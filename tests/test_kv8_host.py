@@ -388,3 +388,21 @@ def test_library_is_linked_without_the_native_module(monkeypatch, tmp_path):
     with pytest.raises(RuntimeError, match="Python.h"):
         build.build_library(verbose=False)
     assert linked == [build.LIB_PATH, build.DIAG_LIB_PATH]
+
+
+def test_module_of_another_python_or_torch(monkeypatch, tmp_path):
+    """Its file name carries the interpreter's tag, and one that does not load says what to do."""
+    import sysconfig
+    from morphserve_amd.csrc import build
+    suffix = sysconfig.get_config_var("EXT_SUFFIX")
+    assert build.BINDING_PATH.endswith("_binding" + suffix)
+    monkeypatch.setattr(_capi, "_binding", None)
+    monkeypatch.setattr(_capi, "_HERE", str(tmp_path))
+    (tmp_path / "csrc").mkdir()
+    (tmp_path / "csrc" / "_binding.so").write_bytes(b"of whatever interpreter")
+    with pytest.raises(ImportError, match="is missing: build it"):
+        _capi.binding()
+    (tmp_path / "csrc" / ("_binding" + suffix)).write_bytes(b"no module")
+    for _ in range(2):                                      # a failed load is not taken for the module the next time
+        with pytest.raises(ImportError, match="build it again with"):
+            _capi.binding()
