@@ -406,3 +406,13 @@ def test_module_of_another_python_or_torch(monkeypatch, tmp_path):
     for _ in range(2):                                      # a failed load is not taken for the module the next time
         with pytest.raises(ImportError, match="build it again with"):
             _capi.binding()
+
+
+@pytest.mark.parametrize("bad", [dict(scale=0.0), dict(scale=-0.1), dict(scale=math.nan), dict(scale=-math.inf), dict(o=A + 8), dict(os_=1028)])
+def test_bad_chunk_attention(bad):
+    """What the chunk entry refuses and the decode entry does not."""
+    a = dict(o=A, os_=1024, scale=0.1)
+    a.update(bad)
+    assert _capi.lib().mkv_attn8_prefill(C.byref(pool8()), C.byref(batch8()), 0, A, a["o"], 1024, a["os_"], 8, a["scale"], 0, 64, 2, A, A,
+                                         None) == _capi.MKV_EINVAL
+    assert (b"softmax_scale" if "scale" in bad else b"aligned") in _capi.lib().mkv_last_error()
