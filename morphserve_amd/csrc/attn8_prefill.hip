@@ -156,7 +156,8 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
     constexpr int kRows = 16 * COLS * WAVES;                  // rows of the tile
     constexpr int kX = D / 32, kT = D / 16;                   // steps of the first product, dim tiles of the second
     constexpr int kUnits = 4 * D;                             // 16-byte units of a tile's K (and V) slabs
-    constexpr int kU = kUnits >= kThreads ? kUnits / kThreads : 1;
+    static_assert(kUnits % kThreads == 0, "every thread takes as many units");
+    constexpr int kU = kUnits / kThreads;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -221,7 +222,7 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
     const uint16_t* scales = scale_row8(g.pool, g.layer, kvh);
 
     // ---- staging: unit w of a tile's slabs belongs to block w / D; a thread takes units tid, tid + kThreads, ... ---------
-    auto unit = [&](int u) { return (tid + kThreads * u) % kUnits; };       // more threads than units: some twice
+    auto unit = [&](int u) { return tid + kThreads * u; };
     // Ids are kept as the table holds them and looked at when they are used, a tile later: loads complete in order, and a
     // glance at an id that was just asked for would wait for the codes asked for before it.
     auto ask_id = [&](int blk) { return table[min(blk, nblk - 1)]; };
