@@ -74,3 +74,85 @@ def test_old_codes_behind_the_largest_values(cuda, monkeypatch, dtype, kind, spl
     n = sum(b.chunks)
     assert_within(chunks(b, cuda, q[:n]), *b.expect_chunks(q[:n]), "chunks")
     assert_within(decode(b, cuda, q[n:]), *b.expect_decode(q[n:]), "decode rows")
+
+
+# Launch shapes of chunk attention: rows of a row tile, and whether row tiles go out in pairs or in order of length.  Each takes
+# more row tiles than small batches have.
+EIGHT = dict(hq=32, hkv=32, chunks=[400, 300, 130, 390, 257, 65, 512, 128], prefixes=[0, 17, 5, 30, 0, 29, 1, 9])
+FIVE = dict(hq=64, hkv=64, dim=64, chunks=[520, 257, 130, 65, 513], prefixes=[3, 17, 0, 30, 1])
+WIDE = dict(hq=64, hkv=64, chunks=[520, 513, 257], prefixes=[3, 17, 0])
+SORTED = dict(hq=64, hkv=64, chunks=[60, 520, 300], prefixes=[2000, 0, 40])
+ALONE = dict(hq=64, hkv=64, chunks=[520, 300], prefixes=[0, 5])
+SHAPES = {"128 rows in pairs": EIGHT, "128 rows of 64 dims in pairs": FIVE, "256 rows in pairs": WIDE, "256 rows by length": SORTED,
+          "256 rows": ALONE}
+
+
+def shaped(name, dtype, kind):
+    """A batch of the shape, its cached codes drawn and not rounded from values: quick for many heads."""
+    b = Batch(62, dtype=dtype, kind=kind, layers=1, layer=0, live="before", **SHAPES[name])
+    top = 0x60 if kind == "e4m3" else 0x80                  # e4m3: up to 32, no NaN
+    b.kc, b.vc = b.kc % top, b.vc % top
+    for x in (b.kc, b.vc):
+        x |= b.rng.integers(0, 2, x.shape, dtype=np.uint8) << 7
+    b.scales = b.rng.integers(120, 125, b.scales.shape, dtype=np.uint8) - (0 if kind == "e4m3" else 2)
+    return b
+
+
+def check_shape(name, b, cuda):
+    """The batch takes the launch shape that its name says, on this card."""
+    units = torch.cuda.get_device_properties(cuda).multi_processor_count
+    rows, per = max(b.chunks) * (b.hq // b.hkv), int(name.split()[0])
+    columns = b.hkv * len(b.chunks)
+    cells = columns * -(-rows // per)
+    assert per == (256 if b.dim == 128 and rows > 512 and columns * -(-rows // 256) >= units else 128)
+    by_length = cells > 2 * units and max(b.chunks) + max(b.prefixes) > 31 * 64
+    assert by_length == ("by length" in name)
+    assert ("in pairs" in name) == (not by_length and cells >= units * (2 if per == 256 else 4 if b.dim == 128 else 6))
+
+
+@pytest.mark.parametrize("name,dtype", zip(SHAPES, itertools.cycle(("bf16", "f16"))))
+def test_shapes(cuda, name, dtype):
+    b = shaped(name, dtype, "int8")
+    check_shape(name, b, cuda)
+    q = b.new_rows(b.hq)
+    assert_within(chunks(b, cuda, q), *b.expect_chunks(q))
+
+
+@pytest.mark.parametrize("name,dtype", zip(SHAPES, itertools.cycle(("f16", "bf16"))))
+def test_nan_reaches_the_rows_that_see_its_key(cuda, name, dtype):
+    """In every launch shape: a NaN among V's codes is in its head dim of the rows at and behind its position, one among K's in
+    every dim of them, and in no other row -- not in those of an earlier row tile that shares its key tile either."""
+    b = shaped(name, dtype, "e4m3")
+    check_shape(name, b, cuda)
+    q = b.new_rows(b.hq)
+    spoiled, codes = np.zeros(q.shape, dtype=bool), []
+    for s, (n, p) in enumerate(zip(b.chunks, b.prefixes)):
+        # around the ends of the row tiles, of key tiles and of the sequence
+        spots = {0, p, p + n - 1, (p + n - 1) // 64 * 64, p + n // 2}
+        spots |= {p + r + d for r in range(128, n, 128) for d in (-1, 0, 1, 30)}
+        for i, pos in enumerate(sorted(x for x in spots if 0 <= x < p + n)):
+            head, dim, in_k = (7 * i + 3 * s) % b.hq, (13 * i + 5 * s) % b.dim, i % 4 == 3
+            pid = b.table[b.seq_ids[s], pos // K.B]
+            array, at = (b.kc, (pid, 0, head, pos % K.B, dim)) if in_k else (b.vc, (pid, 0, head, dim, pos % K.B))
+            array[at] = 0                                   # the rows that do not see it do not care
+            codes.append((array, at, 0x7f if i % 2 else 0xff))
+            first = int(b.starts[s]) + max(pos - p, 0)
+            spoiled[first:int(b.starts[s]) + n, head, slice(None) if in_k else dim] = True
+    want, bound = b.expect_chunks(q)
+    for array, at, code in codes:
+        array[at] = code
+    got = chunks(b, cuda, q)
+    wrong = np.argwhere(torch.isnan(got).cpu().numpy() != spoiled)
+    assert not len(wrong), f"{len(wrong)} values, at {wrong[:4].tolist()}"
+    got[torch.from_numpy(spoiled).to(cuda)] = 0
+    assert_within(got, np.where(spoiled, 0, want), np.where(spoiled, 1, bound))
+
+
+@pytest.mark.parametrize("dtype,kind", TYPES)
+def test_the_same_call_gives_the_same_bits(cuda, dtype, kind):
+    """Partials are joined in one order, whatever the order in which they were made."""
+    b = Batch(64, hq=16, hkv=4, dtype=dtype, kind=kind, chunks=[200, 3, 65], prefixes=[900, 2000, 0], dec=[3000, 70, 1500])
+    q, n = b.new_rows(b.hq), sum(b.chunks)
+    first = chunks(b, cuda, q[:n]), decode(b, cuda, q[n:])
+    for _ in range(10):
+        assert torch.equal(chunks(b, cuda, q[:n]), first[0]) and torch.equal(decode(b, cuda, q[n:]), first[1])
