@@ -390,6 +390,8 @@ int rope(PyObject* const* a, Py_ssize_t count) {
         kos = out_rows_of(ot, "k_out", q, tokens, kv_heads, dim);
         k = kt.const_data_ptr();
         k_out = ot.data_ptr();
+    } else if (a[8] != Py_None) {
+        refuse("k_out without k");
     }
     if (heads > INT32_MAX || kv_heads > INT32_MAX || dim > INT32_MAX) refuse("sizes are out of range");
     const at::Tensor& pos = tensor(a[3], "positions");

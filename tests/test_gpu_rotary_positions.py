@@ -124,3 +124,12 @@ def test_refusals(cuda):
         rotary_embedding(q, None, pos, *rotary_scaled_tables(66, 10, device=cuda))
     torch.cuda.synchronize()
     assert not q.any()
+
+
+def test_an_output_without_its_input_is_refused(cuda):
+    q = torch.ones(4, 2, 64, dtype=torch.float16, device=cuda)
+    k_out = torch.zeros_like(q)
+    with pytest.raises(ValueError):
+        rotary_embedding(q, None, torch.ones(4, dtype=torch.int32, device=cuda), *rotary_scaled_tables(32, 10, device=cuda), k_out=k_out)
+    torch.cuda.synchronize()
+    assert (q == 1).all() and not k_out.any()
