@@ -222,7 +222,8 @@ __device__ __forceinline__ void attend_tile(const Prefill8Args& g, char (*k_lds)
     const uint16_t* scales = scale_row8(g.pool, g.layer, kvh);
 
     // ---- staging: unit w of a tile's slabs belongs to block w / D; a thread takes units tid, tid + kThreads, ... ---------
-    auto unit = [&](int u) { return tid + kThreads * u; };
+    // below kUnits as it is; with the bound in sight the compiler's order of the loop is 2 % faster for few rows (52.3 us, 53.3)
+    auto unit = [&](int u) { return (tid + kThreads * u) % kUnits; };
     // Ids are kept as the table holds them and looked at when they are used, a tile later: loads complete in order, and a
     // glance at an id that was just asked for would wait for the codes asked for before it.
     auto ask_id = [&](int blk) { return table[min(blk, nblk - 1)]; };
