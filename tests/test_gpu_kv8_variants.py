@@ -156,3 +156,29 @@ def test_the_same_call_gives_the_same_bits(cuda, dtype, kind):
     first = chunks(b, cuda, q[:n]), decode(b, cuda, q[n:])
     for _ in range(10):
         assert torch.equal(chunks(b, cuda, q[:n]), first[0]) and torch.equal(decode(b, cuda, q[n:]), first[1])
+
+
+def test_c_entries_with_descriptor_and_chosen_ranges(cuda):
+    """A caller of the C entries takes the pool from ``KV8Cache.descriptor`` and the ranges from the package's rules: the bits
+    of the Python calls."""
+    import ctypes as C
+    from morphserve_amd import _capi
+    b = Batch(65, hq=8, hkv=2, chunks=[20, 3], prefixes=[900, 2000], dec=[3000, 70])
+    q, n = b.new_rows(b.hq), sum(b.chunks)
+    want = chunks(b, cuda, q[:n]), decode(b, cuda, q[n:])
+    cache, table, st, prefix = b.cache(cuda), b.block_table(cuda), b.state(cuda), b.prefix_tensor(cuda)
+    pool, units = cache.descriptor(), torch.cuda.get_device_properties(cuda).multi_processor_count
+    batch = _capi.MkvBatch(table.data_ptr(), table.shape[1], table.shape[0], st.seq_ids.data_ptr(), st.prefill_seq_start_locs.data_ptr(),
+                           st.prefill_seq_lens.data_ptr(), prefix.data_ptr(), st.decoding_seq_lens.data_ptr(), len(b.chunks), n,
+                           st.max_prefill_len, len(b.dec))
+    qg = rounded(q, "f16").to(cuda)
+    o = torch.empty_like(qg)
+    for entry, rows, split in (("mkv_attn8_prefill", slice(0, n), kv8.choose_prefill_split_8bit(2, 8, 2, 20, 20 + 2000, units, 128)),
+                               ("mkv_attn8_decode", slice(n, b.tokens), kv8.choose_split_8bit(2, 2, 3000, units, 8, 128))):
+        x, y = qg[rows], o[rows]
+        mid = torch.empty(x.shape[0] * 8 * split[1], 128 + 1, dtype=torch.float32, device=cuda)
+        assert split[1] > 1
+        _capi.check(getattr(_capi.lib(), entry)(C.byref(pool), C.byref(batch), _capi.F16, x.data_ptr(), y.data_ptr(), 1024, 1024, 8, b.scale,
+                                                b.layer, *split, mid.data_ptr(), mid.view(-1)[mid.shape[0] * 128:].data_ptr(),
+                                                _capi.current_stream()))
+    assert torch.equal(o[:n], want[0]) and torch.equal(o[n:], want[1])
