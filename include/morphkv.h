@@ -479,7 +479,7 @@ int mkv_sizeof_batch(void);
  * 1.875 * 2^127 (bf16) first; a NaN takes no part in the maximum and is stored as a
  * NaN (e4m3) or as 0 (int8).
  * rope != MKV_ROPE_NONE: k is rotated first, in 32 bits and with no rounding before
- * the codes', and q : [rows, Hq, D] is rotated into q_out (which may be q), by row
+ * the codes', and q : [rows, Hq, D] is rotated into q_out (q, or overlapping no input), by row
  * `position` of cos_table / sin_table ([num_positions, rotary_dim / 2] fp32); head
  * dims >= rotary_dim stay as they are.  k itself is not written.  A row whose
  * position lies outside the tables is not appended and its rotated q is NaN.

@@ -20,7 +20,7 @@ import torch
 from ... import _capi
 from ...kv8_cache import KV8Cache
 
-# (tokens_per_split, max_splits) for every attention call instead of the rules below; tests set it
+# (tokens_per_split, max_splits) for every attention call of the process instead of the rules below; tests set it
 FORCED_SPLIT: Optional[Tuple[int, int]] = None
 
 
@@ -58,7 +58,7 @@ def rotary_embedding_and_store_kvcache_8bit(
     infer_state,
     cur_layer: int,
     layout: str = "half",               # or "interleaved", as for rotary_embedding
-    q_out: Optional[torch.Tensor] = None,         # None: q itself
+    q_out: Optional[torch.Tensor] = None,         # None: q itself; otherwise a tensor that overlaps no input
     prefix_lens: Optional[torch.Tensor] = None,
 ) -> None:
     """``rotary_embedding`` of q and k by their positions in the sequences, then ``store_kvcache_8bit``, in one launch.
@@ -72,7 +72,8 @@ def rotary_embedding_and_store_kvcache_8bit(
 def choose_split_8bit(n: int, num_kv_heads: int, max_len: int, units: int = 256, num_q_heads: Optional[int] = None,
                       head_dim: int = 128) -> Tuple[int, int]:
     """``(tokens_per_split, max_splits)`` of a decode launch over ``n`` rows on ``units`` compute units: the ranges with the
-    least estimated time, their joining included."""
+    least estimated time, their joining included.  ``paged_attention_8bit`` takes them so; a caller of ``mkv_attn8_decode``
+    passes them."""
     return _capi.binding().decode_split(n, num_kv_heads, max_len, units, num_q_heads or num_kv_heads, head_dim)
 
 

@@ -56,7 +56,7 @@ def attention_section(
     rotary: bool = True,
     keep_rotated_inputs: bool = False,
     decoding_piggyback_stream: Optional[torch.cuda.Stream] = None,
-    rotary_tables: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,    # 8-bit cache: fp32 (cos, sin) by position
+    rotary_tables: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,    # 8-bit cache: those of rotary_scaled_tables
     rotary_layout: str = "half",                                          # 8-bit cache: "half" or "interleaved"
     prefix_lens: Optional[torch.Tensor] = None,                           # 8-bit cache: cached tokens before each chunk
     max_prefix_len: int = 0,
